@@ -8,6 +8,7 @@
 
 #include <algorithm>
 
+#include "g4_cache.h"
 #include "g4_dkdv_split.h"
 #include "g4_kernels.h"
 
@@ -864,6 +865,72 @@ int g4_tile_ranges(const g4_problem* p, int direction, int row_tile, int32_t* ou
   g4::span_arrays(*p, ws, &lo, &hi);
   hipError_t e = g4::launch_ranges(*p, direction, row_tile, out, lo, hi, st);
   if (e != hipSuccess) return hip_fail(e, "ranges");
+  return G4_OK;
+}
+
+// ---- the paged cache held in 8 bits ---------------------------------------
+
+static int check_cache(const g4_paged_cache* c) {
+  if (c == nullptr) return fail(G4_ERR_INVALID, "cache descriptor is NULL");
+  if (c->head_dim != 256 && c->head_dim != 512)
+    return fail(G4_ERR_UNSUPPORTED, "cache head_dim must be 256 or 512");
+  if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
+    return fail(G4_ERR_UNSUPPORTED, "cache page_size must be 32, 64, 128 or 256");
+  if (c->num_pages < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 65535)
+    return fail(G4_ERR_INVALID, "num_pages and num_kv_heads must be positive (heads below 65536)");
+  if (c->k == nullptr || c->v == nullptr || ((uintptr_t)c->k) % 16 || ((uintptr_t)c->v) % 16)
+    return fail(G4_ERR_INVALID, "cache k and v must be 16-byte aligned");
+  if (c->k_scale == nullptr || c->v_scale == nullptr || ((uintptr_t)c->k_scale) % 4 ||
+      ((uintptr_t)c->v_scale) % 4)
+    return fail(G4_ERR_INVALID, "cache scales must be 4-byte aligned fp32 arrays");
+  return G4_OK;
+}
+
+static int check_table(const g4_page_table* t) {
+  if (t == nullptr) return fail(G4_ERR_INVALID, "page table descriptor is NULL");
+  if (t->batch < 1 || t->width < 1 || t->batch > (1 << 24))
+    return fail(G4_ERR_INVALID, "page table batch and width must be positive (batch up to 2^24)");
+  if (t->pages == nullptr || t->seq_lens == nullptr)
+    return fail(G4_ERR_INVALID, "page table arrays must not be NULL");
+  return G4_OK;
+}
+
+// Packed rows of a cache call: cu and their number.
+static int check_rows(const int32_t* cu, int64_t total) {
+  if (cu == nullptr) return fail(G4_ERR_INVALID, "cumulative lengths are NULL");
+  if (total < 0 || total > 0x7fffffffLL)
+    return fail(G4_ERR_INVALID, "the number of packed rows must be in [0, 2^31)");
+  return G4_OK;
+}
+
+int g4_cache_append(const g4_paged_cache* cache, const g4_page_table* table, const int32_t* cu,
+                    int64_t total, const void* k, g4_layout kl, const void* v, g4_layout vl,
+                    void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_cache(cache));
+  G4_TRY(check_table(table));
+  G4_TRY(check_rows(cu, total));
+  if (total == 0) return G4_OK;
+  G4_TRY(check_operand(k, kl, "k"));
+  G4_TRY(check_operand(v, vl, "v"));
+  g4::AppendParams a{*cache, *table, cu, total, {(const __bf16*)k, (const __bf16*)v}, {kl, vl}};
+  hipError_t e = g4::launch_cache_append(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "cache append");
+  return G4_OK;
+}
+
+int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table, const int32_t* cu,
+                    int64_t total, void* k, g4_layout kl, void* v, g4_layout vl, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_cache(cache));
+  G4_TRY(check_table(table));
+  G4_TRY(check_rows(cu, total));
+  if (total == 0) return G4_OK;
+  G4_TRY(check_operand(k, kl, "k"));
+  G4_TRY(check_operand(v, vl, "v"));
+  g4::GatherParams a{*cache, *table, cu, total, {(__bf16*)k, (__bf16*)v}, {kl, vl}};
+  hipError_t e = g4::launch_cache_gather(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "cache gather");
   return G4_OK;
 }
 

@@ -40,6 +40,7 @@ from .model_spec import (
     AttentionLayerSpec,
     Gemma4ModelSpec,
 )
+from .paged_cache import PagedKVCache, paged_cache_append, paged_cache_gather
 from .transformers_integration import (
     BACKEND_NAME,
     Gemma4DispatchResult,
@@ -66,6 +67,9 @@ __all__ = [
     "fa4_global_varlen_forward_only",
     "pin_backward_ds_budget",
     "prepare_global_kv_from_projection_source",
+    "PagedKVCache",
+    "paged_cache_append",
+    "paged_cache_gather",
     "GlobalBackwardBudgetExceeded",
     "UnsupportedH100Path",
     "UnsupportedMI355XPath",

@@ -42,6 +42,8 @@ EXPORTED_SYMBOLS = (
     "g4_kv_prep_fwd",
     "g4_kv_prep_workspace_bytes",
     "g4_kv_prep_bwd",
+    "g4_cache_append",
+    "g4_cache_gather",
 )
 
 
@@ -88,10 +90,35 @@ class G4KvPrep(ctypes.Structure):
     ]
 
 
+class G4PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
+class G4PageTable(ctypes.Structure):
+    _fields_ = [
+        ("pages", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _L = G4Layout
 _PROB = ctypes.POINTER(G4Problem)
 _PREP = ctypes.POINTER(G4KvPrep)
+_CACHE = ctypes.POINTER(G4PagedCache)
+_TABLE = ctypes.POINTER(G4PageTable)
+_I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 
 _SIGNATURES = {
@@ -121,6 +148,8 @@ _SIGNATURES = {
         ctypes.c_int,
         [_PREP, _P, _L, _P, _P, _P, _P, _L, _P, _L, _P, _L, _P, _P, _SZ, _P],
     ),
+    "g4_cache_append": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
+    "g4_cache_gather": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,180 @@
+"""A paged K/V cache held in 8 bits, and the operators over it, on gfx950.
+
+The reference decodes against a contiguous bf16 StaticCache
+(``src/gemma4_fa4/h100_torch_ops.py:479-846``); it has no counterpart of this
+cache.  K and V are e4m3 with one fp32 scale, a power of two, for each block of
+32 tokens of a page and KV head, so a token's element is ``value * scale``,
+which bf16 holds exactly.  Token ``t`` of sequence ``b`` lies in row
+``t % page_size`` of page ``page_table[b, t // page_size]``.
+
+* ``PagedKVCache``: one layer's pages.
+* ``paged_cache_append``: round the new tokens' K and V rows into the pages.
+* ``paged_cache_gather``: read tokens back as packed bf16 rows.
+
+The page table, lengths and cumulative arrays stay on the device: no call reads
+them on the host, so every call can be captured in a graph.  A table entry
+outside ``[0, num_pages)`` is no page: nothing is read or written for it.
+Nothing here takes part in autograd.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import G4Layout, G4PagedCache, G4PageTable
+from .attention import _check_real_operands, _empty_as, _require_gfx950, _validate_layout
+from .errors import UnsupportedMI355XPath
+
+CACHE_BLOCK = 32  # tokens that share a scale
+PAGE_SIZES = (32, 64, 128, 256)
+_E4M3 = torch.float8_e4m3fn
+
+
+class PagedKVCache:
+    """One layer's K and V pages: e4m3 tensors and their scales.
+
+    ``k`` / ``v``: ``(num_pages, num_kv_heads, page_size, head_dim)`` float8_e4m3fn,
+    ``k_scale`` / ``v_scale``: ``(num_pages, num_kv_heads, page_size // 32)`` fp32
+    powers of two, all contiguous on one gfx950 device.  ``page_size`` is 32, 64,
+    128 or 256, ``head_dim`` 256 or 512.  The tensors are used as they are, so
+    several handles may share them; what they hold need not be initialised.
+    """
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor):
+        for name, t in (("k", k), ("v", v)):
+            if t.ndim != 4 or t.dtype != _E4M3:
+                raise ValueError(f"cache {name} must be a rank-4 float8_e4m3fn tensor "
+                                 "(num_pages, num_kv_heads, page_size, head_dim)")
+        if v.shape != k.shape:
+            raise ValueError("cache k and v must have the same shape")
+        pages, heads, page_size, head_dim = k.shape
+        if pages < 1 or heads < 1:
+            raise ValueError("a cache needs at least one page and one head")
+        if page_size not in PAGE_SIZES or head_dim not in (256, 512):
+            raise UnsupportedMI355XPath(
+                "the paged cache covers page sizes 32, 64, 128 and 256 and head dims 256 and 512")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or t.shape != (pages, heads, page_size // CACHE_BLOCK):
+                raise ValueError(f"cache {name} must be a float32 tensor "
+                                 "(num_pages, num_kv_heads, page_size // 32)")
+        tensors = (k, v, k_scale, v_scale)
+        if any(t.device != k.device for t in tensors):
+            raise ValueError("the cache's tensors must share a device")
+        if not all(t.is_contiguous() for t in tensors):
+            raise ValueError("the cache's tensors must be contiguous")
+        if len({t.untyped_storage().data_ptr() for t in (k, v)}) != 2:
+            raise ValueError("cache k and v must be distinct tensors")
+        _check_real_operands((k, v), ("k", "v"), label="cache k and v")
+        _require_gfx950(k.device)
+        self.k, self.v, self.k_scale, self.v_scale = tensors
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = k.device
+        self._desc = G4PagedCache(
+            k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            pages, heads, head_dim, page_size)
+
+    @classmethod
+    def empty(cls, num_pages: int, *, num_kv_heads: int, head_dim: int, page_size: int = 64,
+              device="cuda") -> "PagedKVCache":
+        """A cache of uninitialised pages."""
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        scales = (num_pages, num_kv_heads, page_size // CACHE_BLOCK)
+        return cls(*(torch.empty(shape, dtype=_E4M3, device=device) for _ in range(2)),
+                   *(torch.empty(scales, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _ints(t: torch.Tensor, shape, device, name: str) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be an INT32 tensor of shape {shape}")
+    if t.device != device:
+        raise ValueError(f"{name} must share the cache's device")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _table(page_table: torch.Tensor, seq_lens: torch.Tensor, device) -> G4PageTable:
+    if page_table.ndim != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
+        raise ValueError("page_table must be a rank-2 (batch, width) tensor")
+    batch, width = page_table.shape
+    _ints(page_table, (batch, width), device, "page_table")
+    _ints(seq_lens, (batch,), device, "seq_lens")
+    return G4PageTable(page_table.data_ptr(), seq_lens.data_ptr(), batch, width)
+
+
+def _no_autograd(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise UnsupportedMI355XPath("the paged cache cannot participate in autograd")
+
+
+def paged_cache_append(
+    cache: PagedKVCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+) -> None:
+    """Round new K and V rows into the pages of their sequences.
+
+    ``k`` / ``v`` are packed bf16 ``(T, num_kv_heads, head_dim)``; rows
+    ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` are the last tokens of sequence ``b``,
+    counted in ``seq_lens[b]``.  A block's scale is the smallest power of two ``s``
+    with ``amax / s <= 448`` (at least 2^-64); a block that already holds earlier
+    tokens keeps the larger of that and its own, and where it grows they are rounded
+    again.  Infinities are stored as the block's largest value, NaN as zero.  Tokens
+    without a page are dropped, rows past ``cu_seqlens[-1]`` are not read.  A page
+    may receive tokens of one sequence only (``reserve_pages`` sees to that).
+    """
+    if k.ndim != 3 or v.ndim != 3 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("k and v must be rank-3 BF16 (T, H, D) tensors")
+    if k.shape[1:] != (cache.num_kv_heads, cache.head_dim) or v.shape != k.shape:
+        raise ValueError("k and v must match each other and the cache's heads and head dim")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError("k and v must share the cache's device")
+    _no_autograd(k, v)
+    table = _table(page_table, seq_lens, cache.device)
+    _ints(cu_seqlens, (table.batch + 1,), cache.device, "cu_seqlens")
+    if k.shape[0] == 0:
+        return
+    _validate_layout(k, name="k")
+    _validate_layout(v, name="v")
+    _check_real_operands((k, v), ("k", "v"), label="k and v")
+    with _lib.device_scope(cache.device):
+        _lib.check(_lib.load().g4_cache_append(
+            ctypes.byref(cache._desc), ctypes.byref(table), cu_seqlens.data_ptr(), k.shape[0],
+            k.data_ptr(), G4Layout(0, k.stride(0), k.stride(1)),
+            v.data_ptr(), G4Layout(0, v.stride(0), v.stride(1)),
+            _lib.raw_stream(cache.device)))
+
+
+def paged_cache_gather(
+    cache: PagedKVCache,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    total: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The sequences' tokens as packed bf16 ``(total, num_kv_heads, head_dim)`` K and V.
+
+    Row ``cu_seqlens[b] + t`` is token ``t`` of sequence ``b`` (exactly what the cache
+    stands for); rows of tokens past ``seq_lens[b]`` or without a page are zero.
+    Rows past ``cu_seqlens[-1]`` are not written.
+    """
+    if type(total) is not int or total < 0:
+        raise ValueError("total must be a non-negative Python integer")
+    table = _table(page_table, seq_lens, cache.device)
+    _ints(cu_seqlens, (table.batch + 1,), cache.device, "cu_seqlens")
+    k = torch.empty((total, cache.num_kv_heads, cache.head_dim), dtype=torch.bfloat16,
+                    device=cache.device)
+    v = _empty_as(k)
+    if total:
+        layout = G4Layout(0, k.stride(0), k.stride(1))
+        with _lib.device_scope(cache.device):
+            _lib.check(_lib.load().g4_cache_gather(
+                ctypes.byref(cache._desc), ctypes.byref(table), cu_seqlens.data_ptr(), total,
+                k.data_ptr(), layout, v.data_ptr(), layout, _lib.raw_stream(cache.device)))
+    return k, v

@@ -1,7 +1,7 @@
 /*
  * gemma4_attn.h -- C ABI of the MI355X (gfx950) Gemma 4 attention library.
  *
- * Plain C: pointers, sizes and two small POD structs; no torch types.  Every
+ * Plain C: pointers, sizes and a few small POD structs; no torch types.  Every
  * entry point is stream-ordered on the caller's hipStream_t (passed as void*),
  * allocates no device memory (the caller passes a workspace sized by
  * g4_workspace_bytes), performs no host synchronisation, and returns a
@@ -319,6 +319,65 @@ int g4_kv_prep_bwd(const g4_kv_prep* p,
                    float* dweight,
                    void* workspace, size_t workspace_bytes,
                    void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged cache held in 8 bits.  No counterpart in the reference, whose decode
+ * reads a contiguous bf16 StaticCache (src/gemma4_fa4/h100_torch_ops.py:479-846).
+ *
+ * K and V are e4m3 (OCP, largest value 448), (num_pages, num_kv_heads,
+ * page_size, head_dim), contiguous; every G4_CACHE_BLOCK tokens of a page and
+ * head share one fp32 scale, a power of two, in (num_pages, num_kv_heads,
+ * page_size / G4_CACHE_BLOCK) arrays: an element stands for value x scale,
+ * which bf16 holds exactly.  Token t of sequence b lies in row t % page_size of
+ * page pages[b][t / page_size].  A page ID outside [0, num_pages) is no page.
+ */
+#define G4_CACHE_BLOCK 32
+
+typedef struct g4_paged_cache {
+  void* k; /* 16-byte aligned, as v */
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t num_pages;
+  int32_t num_kv_heads;
+  int32_t head_dim;  /* 256 or 512 */
+  int32_t page_size; /* 32, 64, 128 or 256 */
+} g4_paged_cache;
+
+/* Which pages hold the tokens of a batch of sequences. */
+typedef struct g4_page_table {
+  int32_t* pages;    /* device (batch, width) */
+  int32_t* seq_lens; /* device (batch): tokens of each sequence */
+  int32_t batch;
+  int32_t width;
+} g4_page_table;
+
+/*
+ * Round new K and V rows into the cache.  The rows of sequence b are cu[b] ..
+ * cu[b + 1] - 1 of the packed (total, num_kv_heads, head_dim) bf16 operands,
+ * its last tokens: seq_lens[b] counts them.  A block's scale is the smallest
+ * power of two s, at least 2^-64, with amax / s <= 448 over its finite values;
+ * where a block already holds earlier tokens of the sequence it is the larger of
+ * that and the block's own, and those tokens are rounded again by the ratio.
+ * Elements round to the nearest (ties to even); infinities become the largest
+ * value of their sign and NaN zero, so that the cache holds finite numbers only
+ * (a NaN in V would reach queries whose mask excludes it).  Rows for tokens
+ * without a page are dropped; rows past cu[batch] and tokens past seq_lens are
+ * left alone.  A page may hold new tokens of one sequence only.
+ */
+int g4_cache_append(const g4_paged_cache* cache, const g4_page_table* table,
+                    const int32_t* cu, int64_t total,
+                    const void* k, g4_layout k_layout,
+                    const void* v, g4_layout v_layout, void* stream);
+
+/*
+ * The tokens of the sequences back as bf16 rows: row cu[b] + t of the packed
+ * (total, num_kv_heads, head_dim) outputs is token t of sequence b; rows of
+ * tokens past seq_lens[b] or without a page are zero.
+ */
+int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table,
+                    const int32_t* cu, int64_t total,
+                    void* k, g4_layout k_layout, void* v, g4_layout v_layout, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,137 @@
+"""Refusals of the paged cache's calls, on the CPU: each wrong argument is named before a launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+import gemma4_fa4_amd as g4
+from gemma4_fa4_amd import _lib
+from gemma4_fa4_amd import paged_cache as pcm
+
+E4M3 = torch.float8_e4m3fn
+
+
+def tensors(pages=4, heads=2, page=64, d=256):
+    z = dict(dtype=torch.uint8)
+    return [torch.zeros(pages, heads, page, d, **z).view(E4M3),
+            torch.zeros(pages, heads, page, d, **z).view(E4M3),
+            torch.ones(pages, heads, page // 32), torch.ones(pages, heads, page // 32)]
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    return g4.PagedKVCache(*tensors())
+
+
+def test_a_cpu_cache_is_refused():
+    with pytest.raises(g4.UnsupportedMI355XPath, match="GPU tensors"):
+        g4.PagedKVCache(*tensors())
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (lambda t: t.__setitem__(0, t[0].view(torch.uint8)), ValueError, "float8_e4m3fn"),
+    (lambda t: t.__setitem__(1, t[1][0]), ValueError, "rank-4"),
+    (lambda t: t.__setitem__(1, t[1][:2]), ValueError, "same shape"),
+    (lambda t: t.__setitem__(1, t[0]), ValueError, "distinct"),
+    (lambda t: t.__setitem__(2, t[2].double()), ValueError, "k_scale"),
+    (lambda t: t.__setitem__(3, t[3][:, :, :1]), ValueError, "v_scale"),
+])
+def test_cache_tensors(change, error, match, monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    t = tensors()
+    change(t)
+    with pytest.raises(error, match=match):
+        g4.PagedKVCache(*t)
+
+
+@pytest.mark.parametrize("page,d", [(16, 256), (48, 256), (512, 256), (64, 128)])
+def test_page_sizes_and_head_dims(page, d, monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    with pytest.raises(g4.UnsupportedMI355XPath, match="page sizes"):
+        g4.PagedKVCache(*tensors(page=page, d=d))
+
+
+def test_non_contiguous_pages(monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    t = tensors(pages=8)
+    with pytest.raises(ValueError, match="contiguous"):
+        g4.PagedKVCache(t[0][::2], t[1][::2], t[2][::2], t[3][::2])
+
+
+def append_args():
+    k = torch.zeros(5, 2, 256, dtype=torch.bfloat16)
+    i = dict(dtype=torch.int32)
+    return dict(k=k, v=k.clone(), page_table=torch.zeros(3, 4, **i), seq_lens=torch.zeros(3, **i),
+                cu_seqlens=torch.zeros(4, **i))
+
+
+@pytest.mark.parametrize("name,value,error,match", [
+    ("k", torch.zeros(5, 2, 256), ValueError, "BF16"),
+    ("k", torch.zeros(5, 1, 256, dtype=torch.bfloat16), ValueError, "heads and head dim"),
+    ("v", torch.zeros(4, 2, 256, dtype=torch.bfloat16), ValueError, "heads and head dim"),
+    ("v", torch.zeros(5, 2, 512, dtype=torch.bfloat16)[..., ::2], ValueError, "unit last"),
+    ("k", torch.zeros(5, 2, 257, dtype=torch.bfloat16)[..., :256], ValueError, "16-byte"),
+    ("k", torch.zeros(5, 2, 256, dtype=torch.bfloat16, requires_grad=True),
+     g4.UnsupportedMI355XPath, "autograd"),
+    ("page_table", torch.zeros(3, 4, dtype=torch.int64), ValueError, "page_table"),
+    ("page_table", torch.zeros(12, dtype=torch.int32), ValueError, "rank-2"),
+    ("page_table", torch.zeros(3, 0, dtype=torch.int32), ValueError, "rank-2"),
+    ("page_table", torch.zeros(4, 3, dtype=torch.int32).t(), ValueError, "contiguous"),
+    ("seq_lens", torch.zeros(2, dtype=torch.int32), ValueError, "seq_lens"),
+    ("cu_seqlens", torch.zeros(3, dtype=torch.int32), ValueError, "cu_seqlens"),
+])
+def test_append_arguments(cache, name, value, error, match):
+    args = append_args() | {name: value}
+    with pytest.raises(error, match=match):
+        g4.paged_cache_append(cache, **args)
+
+
+def test_gather_arguments(cache):
+    a = append_args()
+    for total in (-1, 2.0, True):
+        with pytest.raises(ValueError, match="total"):
+            g4.paged_cache_gather(cache, a["page_table"], a["seq_lens"], a["cu_seqlens"], total)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        g4.paged_cache_gather(cache, a["page_table"], a["seq_lens"], a["seq_lens"], 1)
+
+
+def library_args(**change):
+    """Descriptors for calls that must return before they touch the device."""
+    t = torch.zeros(64, dtype=torch.uint8).data_ptr()
+    t += -t % 16
+    c = dict(k=t, v=t, k_scale=t, v_scale=t, num_pages=4, num_kv_heads=2, head_dim=256, page_size=64)
+    p = dict(pages=t, seq_lens=t, batch=3, width=4)
+    for name, value in change.items():
+        (c if name in c else p)[name] = value
+    return _lib.G4PagedCache(**c), _lib.G4PageTable(**p), t
+
+
+@pytest.mark.parametrize("change,rc", [
+    (dict(head_dim=128), _lib.G4_ERR_UNSUPPORTED), (dict(page_size=48), _lib.G4_ERR_UNSUPPORTED),
+    (dict(num_pages=0), _lib.G4_ERR_INVALID), (dict(num_kv_heads=0), _lib.G4_ERR_INVALID),
+    (dict(k=None), _lib.G4_ERR_INVALID), (dict(k_scale=None), _lib.G4_ERR_INVALID),
+    (dict(batch=0), _lib.G4_ERR_INVALID), (dict(width=0), _lib.G4_ERR_INVALID),
+    (dict(pages=None), _lib.G4_ERR_INVALID), (dict(seq_lens=None), _lib.G4_ERR_INVALID),
+])
+def test_the_library_refuses(change, rc):
+    lib = _lib.load()
+    cache, table, t = library_args(**change)
+    lay = _lib.G4Layout(0, 512, 256)
+    args = [ctypes.byref(cache), ctypes.byref(table), t, 5, t, lay, t, lay, None]
+    assert lib.g4_cache_append(*args) == rc and lib.g4_last_error()
+    assert lib.g4_cache_gather(*args) == rc
+
+
+def test_the_library_refuses_operands():
+    lib = _lib.load()
+    cache, table, t = library_args()
+    good, bad = _lib.G4Layout(0, 512, 256), _lib.G4Layout(0, 512, 4)
+    for call in (lib.g4_cache_append, lib.g4_cache_gather):
+        head = [ctypes.byref(cache), ctypes.byref(table)]
+        assert call(*head, None, 5, t, good, t, good, None) == _lib.G4_ERR_INVALID
+        assert call(*head, t, -1, t, good, t, good, None) == _lib.G4_ERR_INVALID
+        assert call(*head, t, 5, t + 8, good, t, good, None) == _lib.G4_ERR_INVALID
+        assert call(*head, t, 5, t, good, t, bad, None) == _lib.G4_ERR_INVALID
+        assert call(*head, t, 0, None, good, None, good, None) == _lib.G4_OK  # nothing to do
