@@ -934,4 +934,107 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table, con
   return G4_OK;
 }
 
+// ---- page tables and reference counts --------------------------------------
+
+size_t g4_pages_workspace_bytes(int32_t num_pages, int32_t batch, int32_t width) {
+  g_last_error.clear();
+  if (num_pages < 1 || batch < 1 || width < 1) {
+    fail(G4_ERR_INVALID, "num_pages, batch and width must be positive");
+    return 0;
+  }
+  return g4::pages_workspace_bytes(num_pages, batch, width);
+}
+
+// The checks that the calls on the tables share; ws_needed: whether they use a workspace.
+static int check_pages(const g4_page_table* table, const int32_t* refs, int32_t num_pages,
+                       const void* ws, size_t ws_bytes, bool ws_needed) {
+  G4_TRY(check_table(table));
+  if (num_pages < 1) return fail(G4_ERR_INVALID, "num_pages must be positive");
+  if (refs == nullptr) return fail(G4_ERR_INVALID, "ref_counts is NULL");
+  if ((int64_t)table->batch * table->width > 0x7fffffffLL)
+    return fail(G4_ERR_UNSUPPORTED, "the page table must have fewer than 2^31 entries");
+  if (ws_needed) {
+    const size_t need = g4::pages_workspace_bytes(num_pages, table->batch, table->width);
+    if (ws == nullptr || ws_bytes < need || ((uintptr_t)ws) % 256) {
+      char buf[128];
+      snprintf(buf, sizeof buf, "%zu bytes at 256 needed, %zu given", need, ws_bytes);
+      return fail(G4_ERR_WORKSPACE, "page workspace: %s", buf);
+    }
+  }
+  return G4_OK;
+}
+
+static int check_page_size(int32_t page_size) {
+  if (page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+    return fail(G4_ERR_UNSUPPORTED, "page_size must be 32, 64, 128 or 256");
+  return G4_OK;
+}
+
+int g4_pages_fork(const g4_page_table* table, int32_t* refs, int32_t num_pages, int32_t page_size,
+                  const int32_t* parents, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_pages(table, refs, num_pages, ws, ws_bytes, true));
+  G4_TRY(check_page_size(page_size));
+  if (parents == nullptr) return fail(G4_ERR_INVALID, "parents is NULL");
+  g4::PagesParams a{*table, refs, num_pages, page_size, parents};
+  a.ws = (int*)ws;
+  hipError_t e = g4::launch_pages_fork(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page fork");
+  return G4_OK;
+}
+
+int g4_pages_reserve(const g4_page_table* table, int32_t* refs, int32_t num_pages,
+                     int32_t page_size, const int32_t* new_lens, int32_t* src, int32_t* dst,
+                     int32_t* granted, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_pages(table, refs, num_pages, ws, ws_bytes, true));
+  G4_TRY(check_page_size(page_size));
+  if (new_lens == nullptr || src == nullptr || dst == nullptr || granted == nullptr)
+    return fail(G4_ERR_INVALID, "new_lens, src, dst and granted must not be NULL");
+  g4::PagesParams a{*table, refs, num_pages, page_size, new_lens, 0, 0, src, dst, granted,
+                    (int*)ws};
+  hipError_t e = g4::launch_pages_reserve(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page reserve");
+  return G4_OK;
+}
+
+int g4_pages_release(const g4_page_table* table, int32_t* refs, int32_t num_pages,
+                     int32_t page_size, const int32_t* keep_lens, int32_t window,
+                     int32_t num_sinks, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_pages(table, refs, num_pages, nullptr, 0, false));
+  G4_TRY(check_page_size(page_size));
+  if (keep_lens == nullptr) return fail(G4_ERR_INVALID, "keep_lens is NULL");
+  if (window < 0 || num_sinks < 0)
+    return fail(G4_ERR_INVALID, "window and num_sinks must be >= 0");
+  g4::PagesParams a{*table, refs, num_pages, page_size, keep_lens, window, num_sinks};
+  hipError_t e = g4::launch_pages_release(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page release");
+  return G4_OK;
+}
+
+int g4_pages_compact(const g4_page_table* table, int32_t* refs, int32_t num_pages, int32_t* src,
+                     int32_t* dst, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_pages(table, refs, num_pages, ws, ws_bytes, true));
+  if (src == nullptr || dst == nullptr) return fail(G4_ERR_INVALID, "src and dst must not be NULL");
+  g4::PagesParams a{*table, refs, num_pages, 0, nullptr, 0, 0, src, dst, nullptr, (int*)ws};
+  hipError_t e = g4::launch_pages_compact(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page compaction");
+  return G4_OK;
+}
+
+int g4_pages_copy(const g4_paged_cache* cache, const int32_t* src, const int32_t* dst,
+                  int32_t count, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_cache(cache));
+  if (count < 0) return fail(G4_ERR_INVALID, "count must be >= 0");
+  if (count == 0) return G4_OK;
+  if (src == nullptr || dst == nullptr) return fail(G4_ERR_INVALID, "src and dst must not be NULL");
+  g4::CopyParams a{*cache, src, dst};
+  hipError_t e = g4::launch_pages_copy(a, count, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page copy");
+  return G4_OK;
+}
+
 }  // extern "C"

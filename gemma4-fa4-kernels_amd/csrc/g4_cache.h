@@ -90,4 +90,26 @@ struct GatherParams {
 };
 hipError_t launch_cache_gather(const GatherParams& a, hipStream_t stream);
 
+// A call on the tables; what a call does not use is null or 0.
+struct PagesParams {
+  g4_page_table tab;
+  int* refs;
+  int num_pages, page_size;
+  const int* rows;  // parents, new_lens or keep_lens (batch)
+  int window, sinks;
+  int *src, *dst, *granted;
+  int* ws;
+};
+size_t pages_workspace_bytes(int64_t num_pages, int64_t batch, int64_t width);
+hipError_t launch_pages_fork(const PagesParams& a, hipStream_t stream);
+hipError_t launch_pages_reserve(const PagesParams& a, hipStream_t stream);
+hipError_t launch_pages_release(const PagesParams& a, hipStream_t stream);
+hipError_t launch_pages_compact(const PagesParams& a, hipStream_t stream);
+
+struct CopyParams {
+  g4_paged_cache c;
+  const int *src, *dst;
+};
+hipError_t launch_pages_copy(const CopyParams& a, int count, hipStream_t stream);
+
 }  // namespace g4

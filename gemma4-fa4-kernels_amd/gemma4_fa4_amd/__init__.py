@@ -32,6 +32,7 @@ from .facades import (
     gemma4_fa4_compile_layer,
     gemma4_mi355x_compile_layer,
 )
+from .cache_pages import compact_pages, copy_pages, fork_pages, release_pages, reserve_pages
 from .kv_prep import prepare_global_kv_from_projection_source
 from .model_spec import (
     GEMMA4_31B,
@@ -70,6 +71,11 @@ __all__ = [
     "PagedKVCache",
     "paged_cache_append",
     "paged_cache_gather",
+    "fork_pages",
+    "reserve_pages",
+    "release_pages",
+    "compact_pages",
+    "copy_pages",
     "GlobalBackwardBudgetExceeded",
     "UnsupportedH100Path",
     "UnsupportedMI355XPath",

@@ -44,6 +44,12 @@ EXPORTED_SYMBOLS = (
     "g4_kv_prep_bwd",
     "g4_cache_append",
     "g4_cache_gather",
+    "g4_pages_workspace_bytes",
+    "g4_pages_fork",
+    "g4_pages_reserve",
+    "g4_pages_release",
+    "g4_pages_compact",
+    "g4_pages_copy",
 )
 
 
@@ -118,6 +124,7 @@ _PROB = ctypes.POINTER(G4Problem)
 _PREP = ctypes.POINTER(G4KvPrep)
 _CACHE = ctypes.POINTER(G4PagedCache)
 _TABLE = ctypes.POINTER(G4PageTable)
+_I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 
@@ -150,6 +157,13 @@ _SIGNATURES = {
     ),
     "g4_cache_append": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
     "g4_cache_gather": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
+    "g4_pages_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
+    "g4_pages_fork": (ctypes.c_int, [_TABLE, _P, _I32, _I32, _P, _P, _SZ, _P]),
+    "g4_pages_reserve": (
+        ctypes.c_int, [_TABLE, _P, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "g4_pages_release": (ctypes.c_int, [_TABLE, _P, _I32, _I32, _P, _I32, _I32, _P]),
+    "g4_pages_compact": (ctypes.c_int, [_TABLE, _P, _I32, _P, _P, _P, _SZ, _P]),
+    "g4_pages_copy": (ctypes.c_int, [_CACHE, _P, _P, _I32, _P]),
 }
 
 _lock = threading.Lock()

@@ -96,11 +96,13 @@ def _ints(t: torch.Tensor, shape, device, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
-def _table(page_table: torch.Tensor, seq_lens: torch.Tensor, device) -> G4PageTable:
+def _table(page_table: torch.Tensor, seq_lens: torch.Tensor | None, device) -> G4PageTable:
     if page_table.ndim != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
         raise ValueError("page_table must be a rank-2 (batch, width) tensor")
     batch, width = page_table.shape
     _ints(page_table, (batch, width), device, "page_table")
+    if seq_lens is None:
+        return G4PageTable(page_table.data_ptr(), page_table.data_ptr(), batch, width)
     _ints(seq_lens, (batch,), device, "seq_lens")
     return G4PageTable(page_table.data_ptr(), seq_lens.data_ptr(), batch, width)
 

@@ -379,6 +379,53 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table,
                     const int32_t* cu, int64_t total,
                     void* k, g4_layout k_layout, void* v, g4_layout v_layout, void* stream);
 
+/*
+ * Page tables and reference counts (device int32, changed in place).  A page is
+ * free when its count is 0; a sequence uses the first ceil(seq_len / page_size)
+ * entries of its row, -1 standing for no page.  Results do not depend on the
+ * order of atomics.  Workspace: g4_pages_workspace_bytes, 256-byte aligned.
+ */
+size_t g4_pages_workspace_bytes(int32_t num_pages, int32_t batch, int32_t width);
+
+/* Row b becomes a copy of row parents[b] as it was before the call, sharing its
+ * pages; parents[b] == b leaves the row, any value outside [0, batch) empties it. */
+int g4_pages_fork(const g4_page_table* table, int32_t* ref_counts, int32_t num_pages,
+                  int32_t page_size, const int32_t* parents,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row b grows to new_lens[b] tokens (left alone where that is not more).  In the
+ * order of the rows, each takes the lowest free pages: first one for its last page,
+ * where that is part full and shared (the pair src[b], dst[b] says what to copy
+ * before the next append; -1, -1 otherwise), then its new entries.  Of rows that
+ * hold the same part-full page and all of its references, the first keeps it.
+ * granted[b] = 0 where the free pages or the table's width did not suffice: such a
+ * row is left as it was. */
+int g4_pages_reserve(const g4_page_table* table, int32_t* ref_counts, int32_t num_pages,
+                     int32_t page_size, const int32_t* new_lens,
+                     int32_t* src, int32_t* dst, int32_t* granted,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row b keeps its first min(seq_len, max(keep_lens[b], 0)) tokens; pages past them
+ * are given back, and with window > 0 also those whose tokens are neither sinks nor
+ * visible to a query at position keep_lens[b] or later. */
+int g4_pages_release(const g4_page_table* table, int32_t* ref_counts, int32_t num_pages,
+                     int32_t page_size, const int32_t* keep_lens, int32_t window,
+                     int32_t num_sinks, void* stream);
+
+/* The n pages in use move to the first n: pair i of (src, dst), arrays of
+ * max(num_pages / 2, 1) entries padded with -1, is the i-th lowest page in use past
+ * them and the i-th lowest free one among them; tables and counts are rewritten,
+ * contents left to g4_pages_copy.  Lengths are not read. */
+int g4_pages_compact(const g4_page_table* table, int32_t* ref_counts, int32_t num_pages,
+                     int32_t* src, int32_t* dst,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copy page src[i] to page dst[i] (K, V and scales, every head) for every pair of
+ * pages; pairs with an ID outside [0, num_pages) are skipped.  No page may be a
+ * destination twice, or a source and a destination. */
+int g4_pages_copy(const g4_paged_cache* cache, const int32_t* src, const int32_t* dst,
+                  int32_t count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,3 +135,75 @@ def test_the_library_refuses_operands():
         assert call(*head, t, 5, t + 8, good, t, good, None) == _lib.G4_ERR_INVALID
         assert call(*head, t, 5, t, good, t, bad, None) == _lib.G4_ERR_INVALID
         assert call(*head, t, 0, None, good, None, good, None) == _lib.G4_OK  # nothing to do
+
+
+def pool_args():
+    i = dict(dtype=torch.int32)
+    return dict(page_table=torch.zeros(3, 4, **i), seq_lens=torch.zeros(3, **i),
+                ref_counts=torch.zeros(6, **i))
+
+
+ROWS = {g4.fork_pages: "parents", g4.reserve_pages: "new_lens", g4.release_pages: "keep_lens"}
+
+
+@pytest.mark.parametrize("call", list(ROWS), ids=lambda c: c.__name__)
+@pytest.mark.parametrize("name,value,error,match", [
+    ("page_table", torch.zeros(3, 4), ValueError, "page_table"),
+    ("seq_lens", torch.zeros(4, dtype=torch.int32), ValueError, "seq_lens"),
+    ("ref_counts", torch.zeros(6, dtype=torch.int64), ValueError, "ref_counts"),
+    ("ref_counts", torch.zeros(0, dtype=torch.int32), ValueError, "ref_counts"),
+    ("rows", torch.zeros(2, dtype=torch.int32), ValueError, "must be an INT32 tensor"),
+    ("page_size", 48, g4.UnsupportedMI355XPath, "page_size"),
+    (None, None, g4.UnsupportedMI355XPath, "GPU tensors"),
+])
+def test_pool_arguments(call, name, value, error, match):
+    args = pool_args() | {"rows": torch.zeros(3, dtype=torch.int32), "page_size": 64}
+    if name:
+        args[name] = value
+    args[ROWS[call]] = args.pop("rows")
+    with pytest.raises(error, match=match):
+        call(**args)
+
+
+def test_pool_tensors_may_not_be_one():
+    a = pool_args()
+    with pytest.raises(ValueError, match="distinct"):
+        g4.reserve_pages(**a, new_lens=a["seq_lens"], page_size=64)
+
+
+def test_release_window_compact_and_copy_arguments(cache):
+    a = pool_args()
+    keep = torch.zeros(3, dtype=torch.int32)
+    for bad in (dict(sliding_window=0), dict(num_sinks=-1)):
+        with pytest.raises(ValueError):
+            g4.release_pages(**a, keep_lens=keep, page_size=64, **bad)
+    with pytest.raises(ValueError, match="ref_counts"):
+        g4.compact_pages(a["page_table"], a["ref_counts"].long())
+    with pytest.raises(g4.UnsupportedMI355XPath, match="GPU tensors"):
+        g4.compact_pages(a["page_table"][:1].contiguous(), a["ref_counts"])
+    i = torch.zeros(3, dtype=torch.int32)
+    for src, dst in ((i.long(), i), (i, i[:2]), (i[None], i)):
+        with pytest.raises(ValueError, match="src|dst"):
+            g4.copy_pages(cache, src, dst)
+
+
+def test_the_library_refuses_pool_calls():
+    lib = _lib.load()
+    _, table, t = library_args()
+    t += -t % 256
+    assert lib.g4_pages_workspace_bytes(0, 1, 1) == 0 and lib.g4_last_error()
+    need = lib.g4_pages_workspace_bytes(6, 3, 4)
+    assert need >= 3 * 6 * 4
+    ref = ctypes.byref(table)
+    assert lib.g4_pages_fork(ref, t, 6, 64, t, t, need - 1, None) == _lib.G4_ERR_WORKSPACE
+    assert lib.g4_pages_fork(ref, t, 6, 64, t, t + 4, need, None) == _lib.G4_ERR_WORKSPACE
+    assert lib.g4_pages_fork(ref, t, 6, 64, None, t, need, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_fork(ref, None, 6, 64, t, t, need, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_reserve(ref, t, 6, 64, t, None, t, t, t, need, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_reserve(ref, t, 6, 40, t, t, t, t, t, need, None) == _lib.G4_ERR_UNSUPPORTED
+    assert lib.g4_pages_release(ref, t, 6, 64, t, -1, 0, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_compact(ref, t, 0, t, t, t, need, None) == _lib.G4_ERR_INVALID
+    cache, _, _ = library_args()
+    assert lib.g4_pages_copy(ctypes.byref(cache), t, t, -1, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_copy(ctypes.byref(cache), None, t, 1, None) == _lib.G4_ERR_INVALID
+    assert lib.g4_pages_copy(ctypes.byref(cache), None, None, 0, None) == _lib.G4_OK
