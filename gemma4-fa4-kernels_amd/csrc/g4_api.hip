@@ -934,6 +934,73 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table, con
   return G4_OK;
 }
 
+static int check_cache_attn(const g4_cache_attn* p) {
+  if (p == nullptr) return fail(G4_ERR_INVALID, "cache attention descriptor is NULL");
+  G4_TRY(check_cache(&p->cache));
+  G4_TRY(check_table(&p->table));
+  G4_TRY(check_rows(p->cu_seqlens_q, p->total_q));
+  const int hkv = p->cache.num_kv_heads;
+  if (p->num_q_heads < 1 || p->num_q_heads % hkv)
+    return fail(G4_ERR_INVALID, "num_q_heads must be a positive multiple of num_kv_heads");
+  const int grp = p->num_q_heads / hkv;
+  if (grp != 1 && grp != 2 && grp != 4 && grp != 8)
+    return fail(G4_ERR_UNSUPPORTED, "GQA ratio (num_q_heads / num_kv_heads) must be 1, 2, 4 or 8");
+  if (p->max_seqlen_q < 1 || p->max_seqlen_k < 1 || p->max_seqlen_k > (1 << 30) ||
+      p->max_seqlen_q > (1 << 30))
+    return fail(G4_ERR_INVALID, "max_seqlen_q and max_seqlen_k must be in [1, 2^30]");
+  if (p->window < 0 || p->num_sinks < 0)
+    return fail(G4_ERR_INVALID, "window and num_sinks must be >= 0");
+  if (p->num_sinks > G4_MAX_SINKS) return fail(G4_ERR_UNSUPPORTED, "num_sinks must be at most 32");
+  if (p->cache.head_dim == 512 && (p->window > 0 || p->num_sinks > 0))
+    return fail(G4_ERR_UNSUPPORTED, "head_dim 512 attends without a window and sinks");
+  if (p->num_sinks > 0 && p->window == 0)
+    return fail(G4_ERR_INVALID, "num_sinks needs a window");
+  return G4_OK;
+}
+
+static g4::CacheAttnParams cache_attn_params(const g4_cache_attn& p) {
+  g4::CacheAttnParams a{p.cache, p.table, p.cu_seqlens_q, p.total_q, p.num_q_heads};
+  a.max_q = p.max_seqlen_q;
+  a.max_k = p.max_seqlen_k;
+  a.window = p.window;
+  a.sinks = p.num_sinks;
+  a.group_queries = 16 / (p.num_q_heads / p.cache.num_kv_heads);
+  a.groups = (p.max_seqlen_q + a.group_queries - 1) / a.group_queries;
+  return a;
+}
+
+size_t g4_cache_attn_workspace_bytes(const g4_cache_attn* p) {
+  g_last_error.clear();
+  if (check_cache_attn(p) != G4_OK) return 0;
+  return align256(g4::cache_part_bytes(cache_attn_params(*p)));
+}
+
+int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void* o, g4_layout ol,
+                      float* lse, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_cache_attn(p));
+  if (p->total_q == 0) return G4_OK;
+  G4_TRY(check_operand(q, ql, "q"));
+  G4_TRY(check_operand(o, ol, "o"));
+  if (lse == nullptr) return fail(G4_ERR_INVALID, "lse is NULL");
+  g4::CacheAttnParams a = cache_attn_params(*p);
+  const size_t need = align256(g4::cache_part_bytes(a));
+  if (ws == nullptr || ws_bytes < need || ((uintptr_t)ws) % 256) {
+    char buf[128];
+    snprintf(buf, sizeof buf, "%zu bytes at 256 needed, %zu given", need, ws_bytes);
+    return fail(G4_ERR_WORKSPACE, "cache attention workspace: %s", buf);
+  }
+  a.q = (const __bf16*)q;
+  a.o = (__bf16*)o;
+  a.lse = lse;
+  a.ql = ql;
+  a.ol = ol;
+  a.part = (float*)ws;
+  hipError_t e = g4::launch_cache_attn(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "cache attention");
+  return G4_OK;
+}
+
 // ---- page tables and reference counts --------------------------------------
 
 size_t g4_pages_workspace_bytes(int32_t num_pages, int32_t batch, int32_t width) {

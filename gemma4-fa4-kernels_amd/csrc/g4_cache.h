@@ -90,6 +90,25 @@ struct GatherParams {
 };
 hipError_t launch_cache_gather(const GatherParams& a, hipStream_t stream);
 
+// Attention of new tokens over the cached ones.
+struct CacheAttnParams {
+  g4_paged_cache c;
+  g4_page_table tab;
+  const int* cu_q;
+  int64_t total_q;
+  int num_q_heads, max_q, max_k, window, sinks;
+  const __bf16* q;
+  __bf16* o;
+  float* lse;
+  g4_layout ql, ol;
+  float* part;         // partial rows of the segments that several parts share
+  int parts;           // workgroups at most (set by the launcher)
+  int groups;          // row groups of a sequence at most
+  int group_queries;   // queries of a group: 16 / (query heads of a KV head)
+};
+size_t cache_part_bytes(const CacheAttnParams& a);
+hipError_t launch_cache_attn(CacheAttnParams a, hipStream_t stream);
+
 // A call on the tables; what a call does not use is null or 0.
 struct PagesParams {
   g4_page_table tab;

@@ -41,7 +41,12 @@ from .model_spec import (
     AttentionLayerSpec,
     Gemma4ModelSpec,
 )
-from .paged_cache import PagedKVCache, paged_cache_append, paged_cache_gather
+from .paged_cache import (
+    PagedKVCache,
+    paged_cache_append,
+    paged_cache_attention,
+    paged_cache_gather,
+)
 from .transformers_integration import (
     BACKEND_NAME,
     Gemma4DispatchResult,
@@ -70,6 +75,7 @@ __all__ = [
     "prepare_global_kv_from_projection_source",
     "PagedKVCache",
     "paged_cache_append",
+    "paged_cache_attention",
     "paged_cache_gather",
     "fork_pages",
     "reserve_pages",

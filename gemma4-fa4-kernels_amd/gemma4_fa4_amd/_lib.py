@@ -44,6 +44,8 @@ EXPORTED_SYMBOLS = (
     "g4_kv_prep_bwd",
     "g4_cache_append",
     "g4_cache_gather",
+    "g4_cache_attn_workspace_bytes",
+    "g4_cache_attn_fwd",
     "g4_pages_workspace_bytes",
     "g4_pages_fork",
     "g4_pages_reserve",
@@ -118,12 +120,27 @@ class G4PageTable(ctypes.Structure):
     ]
 
 
+class G4CacheAttn(ctypes.Structure):
+    _fields_ = [
+        ("cache", G4PagedCache),
+        ("table", G4PageTable),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("total_q", ctypes.c_int64),
+        ("num_q_heads", ctypes.c_int32),
+        ("max_seqlen_q", ctypes.c_int32),
+        ("max_seqlen_k", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("num_sinks", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _L = G4Layout
 _PROB = ctypes.POINTER(G4Problem)
 _PREP = ctypes.POINTER(G4KvPrep)
 _CACHE = ctypes.POINTER(G4PagedCache)
 _TABLE = ctypes.POINTER(G4PageTable)
+_CATTN = ctypes.POINTER(G4CacheAttn)
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
@@ -157,6 +174,8 @@ _SIGNATURES = {
     ),
     "g4_cache_append": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
     "g4_cache_gather": (ctypes.c_int, [_CACHE, _TABLE, _P, _I64, _P, _L, _P, _L, _P]),
+    "g4_cache_attn_workspace_bytes": (ctypes.c_size_t, [_CATTN]),
+    "g4_cache_attn_fwd": (ctypes.c_int, [_CATTN, _P, _L, _P, _L, _P, _P, _SZ, _P]),
     "g4_pages_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
     "g4_pages_fork": (ctypes.c_int, [_TABLE, _P, _I32, _I32, _P, _P, _SZ, _P]),
     "g4_pages_reserve": (

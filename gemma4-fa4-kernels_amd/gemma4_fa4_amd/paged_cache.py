@@ -9,6 +9,8 @@ which bf16 holds exactly.  Token ``t`` of sequence ``b`` lies in row
 
 * ``PagedKVCache``: one layer's pages.
 * ``paged_cache_append``: round the new tokens' K and V rows into the pages.
+* ``paged_cache_attention``: attention of the sequences' last tokens over the pages,
+  with a sliding window and sinks for local layers.
 * ``paged_cache_gather``: read tokens back as packed bf16 rows.
 
 The page table, lengths and cumulative arrays stay on the device: no call reads
@@ -24,8 +26,14 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import G4Layout, G4PagedCache, G4PageTable
-from .attention import _check_real_operands, _empty_as, _require_gfx950, _validate_layout
+from ._lib import G4CacheAttn, G4Layout, G4PagedCache, G4PageTable
+from .attention import (
+    _check_real_operands,
+    _empty_as,
+    _is_python_int,
+    _require_gfx950,
+    _validate_layout,
+)
 from .errors import UnsupportedMI355XPath
 
 CACHE_BLOCK = 32  # tokens that share a scale
@@ -180,3 +188,78 @@ def paged_cache_gather(
                 ctypes.byref(cache._desc), ctypes.byref(table), cu_seqlens.data_ptr(), total,
                 k.data_ptr(), layout, v.data_ptr(), layout, _lib.raw_stream(cache.device)))
     return k, v
+
+
+MAX_SINKS = 32  # first tokens that a windowed layer may keep visible
+_MAX_LENGTH = 1 << 30
+
+
+def paged_cache_attention(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    page_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    *,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    sliding_window: int | None = None,
+    num_sinks: int = 0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of each sequence's last tokens over its cached tokens (scale 1.0).
+
+    ``q`` is packed bf16 ``(T, Hq, head_dim)``; rows ``cu_seqlens_q[b]`` to
+    ``cu_seqlens_q[b + 1]`` are the last tokens of sequence ``b``, whose own K and V
+    are already in the cache (``paged_cache_append``) and counted in ``seq_lens[b]``.
+    A query at position ``a`` sees token ``j <= a``; with ``sliding_window`` W only
+    ``j > a - W`` or ``j < num_sinks`` (up to 32), and pages that no query sees any more
+    may be gone (``release_pages``).  Returns bf16 O like ``q`` and fp32 LSE ``(Hq, T)``:
+    0 and -inf for a query that sees nothing, NaN where a visible token has no page;
+    rows past ``cu_seqlens_q[-1]`` are not written.  ``max_seqlen_q`` and
+    ``max_seqlen_k`` are bounds of the lengths on the device, which no call reads on the
+    host; a batch beyond them gets unspecified rows.  Head dim 512 takes neither
+    window nor sinks; query heads are 1, 2, 4 or 8 times the cache's.
+    """
+    if q.ndim != 3 or q.dtype != torch.bfloat16:
+        raise ValueError("q must be a rank-3 BF16 (T, H, D) tensor")
+    total, heads, head_dim = q.shape
+    if head_dim != cache.head_dim:
+        raise ValueError("q must have the cache's head dim")
+    if heads < 1 or heads % cache.num_kv_heads:
+        raise ValueError("q's heads must be a positive multiple of the cache's")
+    if heads // cache.num_kv_heads not in (1, 2, 4, 8):
+        raise UnsupportedMI355XPath("the validated GQA ratios are 1, 2, 4, and 8")
+    if q.device != cache.device:
+        raise ValueError("q must share the cache's device")
+    if not (_is_python_int(max_seqlen_q) and _is_python_int(max_seqlen_k)):
+        raise TypeError("max_seqlen_q and max_seqlen_k must be Python integers")
+    if not (1 <= max_seqlen_q <= _MAX_LENGTH and 1 <= max_seqlen_k <= _MAX_LENGTH):
+        raise ValueError("max_seqlen_q and max_seqlen_k must be in [1, 2^30]")
+    if sliding_window is not None and sliding_window < 1:
+        raise ValueError("sliding_window must be positive")
+    if not 0 <= num_sinks <= MAX_SINKS:
+        raise UnsupportedMI355XPath("num_sinks must be in [0, 32]")
+    if sliding_window is None and num_sinks:
+        raise ValueError("num_sinks needs a sliding_window")
+    if head_dim == 512 and sliding_window is not None:
+        raise UnsupportedMI355XPath("head dim 512 attends without a window and sinks")
+    _no_autograd(q)
+    table = _table(page_table, seq_lens, cache.device)
+    _ints(cu_seqlens_q, (table.batch + 1,), cache.device, "cu_seqlens_q")
+    out = _empty_as(q)
+    lse = torch.empty((heads, total), dtype=torch.float32, device=q.device)
+    if total == 0:
+        return out, lse
+    _validate_layout(q, name="q")
+    _check_real_operands((q,), ("q",), label="q")
+    lib = _lib.load()
+    prob = G4CacheAttn(cache._desc, table, cu_seqlens_q.data_ptr(), total, heads,
+                       max_seqlen_q, max_seqlen_k, sliding_window or 0, num_sinks)
+    ref = ctypes.byref(prob)
+    ws = torch.empty(lib.g4_cache_attn_workspace_bytes(ref), dtype=torch.uint8, device=q.device)
+    with _lib.device_scope(q.device):
+        _lib.check(lib.g4_cache_attn_fwd(
+            ref, q.data_ptr(), G4Layout(0, q.stride(0), q.stride(1)),
+            out.data_ptr(), G4Layout(0, out.stride(0), out.stride(1)), lse.data_ptr(),
+            ws.data_ptr(), ws.numel(), _lib.raw_stream(q.device)))
+    return out, lse

@@ -380,6 +380,40 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table,
                     void* k, g4_layout k_layout, void* v, g4_layout v_layout, void* stream);
 
 /*
+ * Attention of the last tokens of each sequence over its cached tokens (their
+ * own rows already appended): query i of sequence b, row cu_seqlens_q[b] + i,
+ * sits at position a = seq_lens[b] - (queries of b) + i, and sees token j <= a
+ * with j > a - window (window > 0) or j < num_sinks.  O bf16, LSE fp32 (heads,
+ * total_q); a query that sees no token gets 0 and -inf, one that sees a token
+ * without a page NaN.  Sequences of one to a few queries are read from the pages
+ * as they lie; larger chunks as bf16 rows in the workspace, through the forward
+ * of g4_attn_fwd.  max_seqlen_q / max_seqlen_k bound the batch's (device)
+ * lengths: queries and tokens past them are not read, written or seen.
+ * head_dim 256: any window, num_sinks 0..G4_MAX_SINKS with a window; head_dim
+ * 512: neither.
+ */
+#define G4_MAX_SINKS 32
+
+typedef struct g4_cache_attn {
+  g4_paged_cache cache;
+  g4_page_table table;
+  const int32_t* cu_seqlens_q; /* device (batch + 1) */
+  int64_t total_q;
+  int32_t num_q_heads; /* 1, 2, 4 or 8 times num_kv_heads */
+  int32_t max_seqlen_q;
+  int32_t max_seqlen_k;
+  int32_t window;
+  int32_t num_sinks;
+} g4_cache_attn;
+
+size_t g4_cache_attn_workspace_bytes(const g4_cache_attn* p);
+
+int g4_cache_attn_fwd(const g4_cache_attn* p,
+                      const void* q, g4_layout q_layout,
+                      void* o, g4_layout o_layout, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Page tables and reference counts (device int32, changed in place).  A page is
  * free when its count is 0; a sequence uses the first ceil(seq_len / page_size)
  * entries of its row, -1 standing for no page.  Results do not depend on the

@@ -1,0 +1,223 @@
+"""paged_cache_attention against fp64 over the exact cached values, within derived bounds
+(paged_testutil.check_attention)."""
+
+import numpy as np
+import pytest
+import torch
+
+import gemma4_fa4_amd as g4
+from paged_testutil import DEV, check_attention, cu_of, empty_cache, filled_cache, ints, queries
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(q, cache, table, lens, new, *, window=0, sinks=0, max_q=None, max_k=None):
+    return g4.paged_cache_attention(
+        q, cache, ints(table), ints(lens), ints(cu_of(new)), max_seqlen_q=max_q or max(new),
+        max_seqlen_k=max_k or max(max(lens), 1), sliding_window=window or None, num_sinks=sinks)
+
+
+def run(seed, d, hkv, grp, page, lens, new, window=0, sinks=0, **kw):
+    print(seed, d, hkv, grp, page, lens[:8], new[:8], window, sinks, flush=True)
+    cache, table = filled_cache(seed, lens, hkv, page, d)
+    q = queries(seed, sum(new), hkv * grp, d)
+    out, lse = attend(q, cache, table, lens, new, window=window, sinks=sinks, **kw)
+    check_attention(q, cache, table, lens, new, out, lse, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("d,hkv,grp,page,lens,new", [
+    (512, 4, 8, 64, [1], [1]),
+    (512, 4, 8, 64, [33], [1]),
+    (512, 4, 8, 32, [700, 31, 2049, 64], [1, 1, 1, 1]),
+    (512, 1, 8, 256, [5000], [1]),
+    (512, 2, 1, 128, [100, 257], [1, 1]),  # GQA 1
+    (512, 1, 2, 64, [300], [8]),  # a whole group of 16 rows
+    (512, 1, 4, 64, [300, 90], [7, 3]),  # two groups, the second part full
+    (512, 4, 8, 64, [515, 12, 200], [5, 0, 12]),  # three groups, none, six
+    (256, 16, 2, 64, [900], [1]),
+    (256, 3, 2, 32, [130, 1, 500], [3, 1, 17]),
+    (256, 2, 8, 128, [77, 40], [40, 40]),
+])
+def test_over_everything(d, hkv, grp, page, lens, new):
+    run(d + page + sum(lens), d, hkv, grp, page, lens, new)
+
+
+@pytest.mark.parametrize("window,sinks,lens,new", [
+    (1024, 4, [3000], [1]),
+    (1024, 0, [3000, 500, 1025], [1, 1, 1]),
+    (1024, 31, [1500, 1056, 1023], [5, 1, 9]),
+    (100, 32, [400, 131, 132, 133], [1, 1, 1, 1]),  # the window's first tile holds sinks too
+    (33, 5, [500, 37, 38, 39, 70], [20, 1, 1, 1, 2]),
+    (1, 1, [64, 2, 1], [4, 1, 1]),
+    (1, 0, [64, 2, 1], [33, 2, 1]),
+    (40, 32, [20, 400], [20, 300]),
+])
+@pytest.mark.parametrize("page", [32, 128])
+def test_windows_and_sinks(window, sinks, lens, new, page):
+    run(window + sinks, 256, 2, 2, page, lens, new, window, sinks)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(seed):
+    rng = np.random.default_rng(1000 + seed)
+    d = int(rng.choice([256, 512]))
+    hkv, grp = int(rng.integers(1, 5)), int(rng.choice([1, 2, 4, 8]))
+    batch = int(rng.integers(1, 12))
+    top = int(rng.choice([40, 300, 2500]))
+    lens = [int(x) for x in rng.integers(1, top, batch)]
+    most = int(rng.choice([1, 3, 30]))
+    new = [min(n, int(x)) for n, x in zip(lens, rng.integers(0, most + 1, batch))]
+    new[0] = max(new[0], 1)
+    window = int(rng.choice([0, 17, 64, 1024])) if d == 256 else 0
+    sinks = int(rng.integers(0, 33)) if window else 0
+    run(seed, d, hkv, grp, int(rng.choice([32, 64, 128, 256])), lens, new, window, sinks,
+        max_q=max(new) + int(rng.integers(0, 3)), max_k=max(lens) + int(rng.integers(0, 200)))
+
+
+def test_hundreds_of_sequences():
+    # more than a workgroup's threads: the batch's prefix sums take several rounds
+    rng = np.random.default_rng(3)
+    lens = [int(x) for x in rng.integers(1, 90, 600)]
+    run(5, 256, 1, 2, 32, lens, [1] * 600, 64, 3)
+
+
+def test_one_long_sequence_among_short_ones():
+    run(6, 512, 2, 8, 64, [40, 20000, 7, 300], [1, 1, 1, 1])
+
+
+def test_large_scores():
+    # maxima that rise by far more than what the softmax absorbs without rescaling
+    cache, table = filled_cache(8, [2000], 1, 64, 512, std_k=4.0)
+    q = queries(8, 1, 8, 512, scale=30.0)
+    out, lse = attend(q, cache, table, [2000], [1])
+    check_attention(q, cache, table, [2000], [1], out, lse)
+
+
+def test_queries_that_see_nothing():
+    # no tokens at all, and more queries than tokens: 0 and -inf
+    cache, table = filled_cache(9, [3, 40], 2, 32, 256)
+    q = queries(9, 9, 4, 256)
+    out, lse = attend(q, cache, table, [3, 0], [5, 4])
+    assert not out[:2].any() and not out[5:].any()
+    assert lse[:, :2].eq(-torch.inf).all() and lse[:, 5:].eq(-torch.inf).all()
+    check_attention(q[2:5], cache, table[:1], [3], [3], out[2:5], lse[:, 2:5])
+
+
+def test_rows_behind_the_last_sequence_stay():
+    cache, table = filled_cache(10, [50], 2, 32, 256)
+    q = queries(10, 6, 4, 256)
+    out, lse = g4.paged_cache_attention(q, cache, ints(table), ints([50]), ints([0, 2]),
+                                        max_seqlen_q=2, max_seqlen_k=50)
+    check_attention(q[:2], cache, table, [50], [2], out[:2], lse[:, :2])
+    assert out[2:].isnan().all() and lse[:, 2:].isnan().all()  # (the fixture's fill)
+
+
+def test_what_lies_past_the_end_and_in_other_pages_is_not_seen():
+    # NaN bytes everywhere but in the tokens: past the last row, in free pages, and in the
+    # pages between the sinks and the window, which are gone from the table
+    lens, new, window, sinks = [333, 61], [2, 1], 64, 3
+    clean, table = filled_cache(11, lens, 2, 32, 256)
+    q = queries(11, 3, 4, 256)
+    want = attend(q, clean, table, lens, new, window=window, sinks=sinks)
+    cache, _ = filled_cache(11, lens, 2, 32, 256)
+    used = torch.zeros(cache.num_pages, 32, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            used[table[b][t // 32], t % 32] = True
+    for t in range(sinks // 32 * 32 + 32, (lens[0] - new[0] - window + 1) // 32 * 32, 32):
+        used[table[0][t // 32]] = False
+        table[0][t // 32] = -1
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).masked_fill_(~used.to(DEV)[:, None, :, None], 0x7F)
+    gone = ~used.any(1).to(DEV)
+    for t in (cache.k_scale, cache.v_scale):
+        t.masked_fill_(gone[:, None, None], float("nan"))
+    got = attend(q, cache, table, lens, new, window=window, sinks=sinks)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+@pytest.mark.parametrize("entry", [-1, 6000, -2147483648, 2147483647])
+def test_a_visible_token_without_a_page_gives_nan(entry):
+    lens, new = [200, 100, 70], [1, 1, 4]
+    cache, table = filled_cache(12, lens, 2, 32, 512)
+    q = queries(12, 6, 4, 512)
+    want, want_lse = attend(q, cache, table, lens, new)
+    table[0][3] = entry
+    table[2][2] = entry  # tokens 64 .. 69: seen by all four queries (positions 66 .. 69)
+    got, lse = attend(q, cache, table, lens, new)
+    assert got[0].isnan().all() and got[2:].isnan().all()
+    assert torch.equal(got[1], want[1]) and torch.equal(lse[:, 1], want_lse[:, 1])
+
+
+def test_a_table_narrower_than_the_lengths():
+    cache, table = filled_cache(13, [64, 64], 1, 32, 256)
+    q = queries(13, 2, 1, 256)
+    out, _ = attend(q, cache, [row[:2] for row in table], [64, 97], [1, 1])
+    assert torch.isfinite(out[0]).all() and out[1].isnan().all()
+
+
+def test_strided_queries_and_another_stream():
+    lens, new = [400, 77], [1, 3]
+    cache, table = filled_cache(14, lens, 2, 64, 256)
+    wide = queries(14, 4, 12, 256)
+    q = wide[:, 4:8]
+    want = attend(q.contiguous(), cache, table, lens, new)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = attend(q, cache, table, lens, new)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_repeats_bitwise():
+    lens, new = [3000, 700, 1], [1, 1, 1]
+    cache, table = filled_cache(15, lens, 4, 64, 512)
+    q = queries(15, 3, 32, 512)
+    first = attend(q, cache, table, lens, new)
+    for _ in range(3):
+        again = attend(q, cache, table, lens, new)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_a_captured_decode_loop():
+    """Reserve, append and attend in one graph, replayed over 44 tokens with eager work
+    between; every replay against the same calls made eagerly on a second cache."""
+    page, hkv, grp, d, window, sinks = 32, 2, 2, 256, 48, 4
+    lens = [70, 5]
+    table = torch.full((2, 6), -1, dtype=torch.int32, device=DEV)
+    state = [(table.clone(), ints([0, 0]), torch.zeros(12, dtype=torch.int32, device=DEV),
+              empty_cache(12, hkv, page, d)) for _ in range(2)]
+    k, v = (queries(20 + i, sum(lens), hkv, d, 16.0) for i in range(2))
+    for t, l, r, cache in state:
+        g4.reserve_pages(t, l, r, ints(lens), page_size=page)
+        g4.paged_cache_append(cache, k, v, t, l, ints(cu_of(lens)))
+    one = ints([0, 1, 2])
+    q, kn, vn = (torch.zeros(2, h, d, dtype=torch.bfloat16, device=DEV) for h in (hkv * grp, hkv, hkv))
+
+    def step(t, l, r, cache, want):
+        src, dst, _ = g4.reserve_pages(t, l, r, want, page_size=page)
+        g4.copy_pages(cache, src, dst)
+        g4.paged_cache_append(cache, kn, vn, t, l, one)
+        out = g4.paged_cache_attention(q, cache, t, l, one, max_seqlen_q=1, max_seqlen_k=192,
+                                       sliding_window=window, num_sinks=sinks)
+        g4.release_pages(t, l, r, want, page_size=page, sliding_window=window, num_sinks=sinks)
+        return out
+
+    target = ints(lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        target.add_(1)
+        got = step(*state[0], target)
+    target.copy_(ints(lens))
+    for i in range(44):
+        for j, x in enumerate((q, kn, vn)):
+            x.copy_(queries(100 + 3 * i + j, 2, x.shape[1], d, 16.0 if j else 1.5))
+        graph.replay()
+        want = step(*state[1], ints([n + i + 1 for n in lens]))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        assert torch.equal(state[0][0], state[1][0]) and torch.equal(state[0][2], state[1][2])
+        # page 1 (tokens 32 .. 63) goes once 63 <= 70 + i + 1 - 48; page 0 holds the sinks
+        assert (state[0][0][0, 1].item() >= 0) == (i < 40)
+    assert state[0][1].tolist() == [n + 44 for n in lens]
+    assert (state[0][0][0] >= 0).tolist() == [True, False, True, True, False, False]

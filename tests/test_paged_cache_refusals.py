@@ -207,3 +207,72 @@ def test_the_library_refuses_pool_calls():
     assert lib.g4_pages_copy(ctypes.byref(cache), t, t, -1, None) == _lib.G4_ERR_INVALID
     assert lib.g4_pages_copy(ctypes.byref(cache), None, t, 1, None) == _lib.G4_ERR_INVALID
     assert lib.g4_pages_copy(ctypes.byref(cache), None, None, 0, None) == _lib.G4_OK
+
+
+def attention_args(d=256, heads=4):
+    i = dict(dtype=torch.int32)
+    return dict(q=torch.zeros(5, heads, d, dtype=torch.bfloat16), page_table=torch.zeros(3, 4, **i),
+                seq_lens=torch.zeros(3, **i), cu_seqlens_q=torch.zeros(4, **i),
+                max_seqlen_q=2, max_seqlen_k=100)
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(q=torch.zeros(5, 4, 256)), ValueError, "BF16"),
+    (dict(q=torch.zeros(5, 4, 512, dtype=torch.bfloat16)), ValueError, "head dim"),
+    (dict(q=torch.zeros(5, 3, 256, dtype=torch.bfloat16)), ValueError, "multiple"),
+    (dict(q=torch.zeros(5, 6, 256, dtype=torch.bfloat16)), g4.UnsupportedMI355XPath, "GQA"),
+    (dict(q=torch.zeros(5, 4, 256, dtype=torch.bfloat16, requires_grad=True)),
+     g4.UnsupportedMI355XPath, "autograd"),
+    (dict(q=torch.zeros(5, 4, 512, dtype=torch.bfloat16)[..., ::2]), ValueError, "unit last"),
+    (dict(max_seqlen_q=0), ValueError, "max_seqlen"),
+    (dict(max_seqlen_k=(1 << 30) + 1), ValueError, "max_seqlen"),
+    (dict(max_seqlen_k=True), TypeError, "integers"),
+    (dict(max_seqlen_q=torch.tensor(2)), TypeError, "integers"),
+    (dict(sliding_window=0), ValueError, "sliding_window"),
+    (dict(num_sinks=4), ValueError, "needs a sliding_window"),
+    (dict(sliding_window=64, num_sinks=33), g4.UnsupportedMI355XPath, "num_sinks"),
+    (dict(sliding_window=64, num_sinks=-1), g4.UnsupportedMI355XPath, "num_sinks"),
+    (dict(cu_seqlens_q=torch.zeros(3, dtype=torch.int32)), ValueError, "cu_seqlens_q"),
+    (dict(seq_lens=torch.zeros(3)), ValueError, "seq_lens"),
+])
+def test_attention_arguments(cache, change, error, match):
+    args = attention_args() | change
+    with pytest.raises(error, match=match):
+        g4.paged_cache_attention(args.pop("q"), cache, **args)
+
+
+def test_attention_of_head_dim_512_takes_no_window(monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    cache = g4.PagedKVCache(*tensors(d=512))
+    args = attention_args(d=512)
+    with pytest.raises(g4.UnsupportedMI355XPath, match="512"):
+        g4.paged_cache_attention(args.pop("q"), cache, **args, sliding_window=64)
+
+
+def test_the_library_refuses_attention():
+    lib = _lib.load()
+    cache, table, t = library_args()
+    t += -t % 256
+    lay = _lib.G4Layout(0, 1024, 256)
+
+    def call(rows=5, ws=None, nbytes=None, q=t, lse=t, **change):
+        p = _lib.G4CacheAttn(cache, table, t, rows, 4, 2, 100, 0, 0)
+        for name, value in change.items():
+            setattr(p, name, value)
+        need = lib.g4_cache_attn_workspace_bytes(ctypes.byref(p))
+        return lib.g4_cache_attn_fwd(ctypes.byref(p), q, lay, t, lay, lse, t if ws is None else ws,
+                                     need if nbytes is None else nbytes, None)
+
+    assert call(num_q_heads=3) == _lib.G4_ERR_INVALID
+    assert call(num_q_heads=32) == _lib.G4_ERR_UNSUPPORTED
+    assert call(max_seqlen_q=0) == _lib.G4_ERR_INVALID
+    assert call(max_seqlen_k=-1) == _lib.G4_ERR_INVALID
+    assert call(window=-1) == _lib.G4_ERR_INVALID
+    assert call(num_sinks=2) == _lib.G4_ERR_INVALID
+    assert call(window=64, num_sinks=33) == _lib.G4_ERR_UNSUPPORTED
+    assert call(cu_seqlens_q=None) == _lib.G4_ERR_INVALID
+    assert call(q=t + 8) == _lib.G4_ERR_INVALID
+    assert call(lse=None) == _lib.G4_ERR_INVALID
+    assert call(nbytes=255) == _lib.G4_ERR_WORKSPACE
+    assert call(ws=t + 16) == _lib.G4_ERR_WORKSPACE
+    assert call(rows=0, q=None, lse=None) == _lib.G4_OK
