@@ -18,7 +18,7 @@ LIB_DIR = os.path.join(HERE, "gemma4_fa4_amd", "_lib")
 LIB = os.path.join(LIB_DIR, "libgemma4_attn.so")
 SOURCES = ["g4_api.hip", "g4_meta.hip", "g4_fwd.hip", "g4_bwd.hip", "g4_bwd_roles.hip",
            "g4_kvprep.hip", "g4_cache.hip", "g4_pages.hip",
-           "g4_cache_attn.hip"]
+           "g4_cache_attn.hip", "g4_sinks.hip"]
 ARCH = "gfx950"
 FLAGS = [
     "-O3",

@@ -194,7 +194,7 @@ int scratch_for_stream(hipStream_t stream, void** out) {
 
 int fwd_impl(const g4_problem* p, const void* q, g4_layout ql, const void* k, g4_layout kl,
              const void* v, g4_layout vl, void* o, g4_layout ol, float* lse, void* ws,
-             size_t ws_bytes, hipStream_t st) {
+             size_t ws_bytes, hipStream_t st, int sinks = 0) {
   g4::FwdParams a{};
   a.p = *p;
   a.q = (const __bf16*)q;
@@ -207,6 +207,14 @@ int fwd_impl(const g4_problem* p, const void* q, g4_layout ql, const void* k, g4
   a.vl = vl;
   a.ol = ol;
   a.num_seqs = p->num_seqs;
+  if (sinks > 0) {  // head dim 256 without key metadata: partial rows are all it may need
+    a.sinks = sinks;
+    a.split_chunks = g4::split_chunks(*p, &a.split_keys, /*extra_tiles=*/1);
+    a.part = a.split_chunks ? (float*)ws : nullptr;
+    hipError_t e = g4::launch_fwd(a, st);
+    if (e != hipSuccess) return hip_fail(e, "forward with sinks");
+    return G4_OK;
+  }
   if (g4::spans_bytes(*p)) {
     hipError_t e = g4::launch_spans(*p, ws, st, /*query_reach=*/false);  // (span_hi only)
     if (e != hipSuccess) return hip_fail(e, "span table");
@@ -415,7 +423,7 @@ size_t raise_flags_bytes(const g4_problem& p) {
 // two rounds of resident workgroups in all (head dim 512: one per CU, 256:
 // two), each chunk a whole number of 32-key tiles, at least four (head dim
 // 512) or two.
-int split_chunks(const g4_problem& p, int* keys) {
+int split_chunks(const g4_problem& p, int* keys, int extra_tiles) {
   if ((p.vision_ids != nullptr && p.bidirectional_vision) || p.document_ids != nullptr) return 0;
   const int64_t rows = (int64_t)(p.num_q_heads / p.num_kv_heads) * p.seqlen_q;
   if (rows > 32) return 0;
@@ -425,7 +433,7 @@ int split_chunks(const g4_problem& p, int* keys) {
   const int64_t target = p.head_dim == 512 ? 512 : 1024;
   const int64_t min_tiles = p.head_dim == 512 ? 4 : 2;
   const int64_t groups = (int64_t)p.num_seqs * p.num_kv_heads;
-  const int64_t tiles = (range + 31) / 32 + 1;  // (the range may start mid-tile)
+  const int64_t tiles = (range + 31) / 32 + 1 + extra_tiles;  // (the range may start mid-tile)
   int64_t n = std::max<int64_t>(1, std::min((target + groups - 1) / groups, tiles / min_tiles));
   const int64_t per = (tiles + n - 1) / n;  // tiles per chunk
   n = (tiles + per - 1) / per;
@@ -533,8 +541,8 @@ size_t dkdv_split_bytes(const g4_problem& p) {
   if (whole <= 1.05 * split) return 0;
   return kDkdvSplitBytes;
 }
-size_t split_bytes(const g4_problem& p) {
-  const int n = split_chunks(p, nullptr);
+size_t split_bytes(const g4_problem& p, int extra_tiles) {
+  const int n = split_chunks(p, nullptr, extra_tiles);
   if (n == 0) return 0;
   const size_t rows = (size_t)(p.num_q_heads / p.num_kv_heads) * p.seqlen_q;
   return align256((size_t)p.num_seqs * p.num_kv_heads * n * rows * (p.head_dim + 2) * 4);
@@ -1101,6 +1109,81 @@ int g4_pages_copy(const g4_paged_cache* cache, const int32_t* src, const int32_t
   g4::CopyParams a{*cache, src, dst};
   hipError_t e = g4::launch_pages_copy(a, count, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "page copy");
+  return G4_OK;
+}
+
+// ---- attention with a window and sinks --------------------------------------
+
+// Key tiles beside the window's: the sinks lie in one 32-key tile.
+static constexpr int kSinkTiles = 1;
+static_assert(G4_MAX_SINKS <= 32, "the sinks lie in one key tile");
+
+static int check_sinks(const g4_problem* p, int32_t num_sinks) {
+  G4_TRY(check_problem(p));
+  if (num_sinks < 1 || num_sinks > G4_MAX_SINKS)
+    return fail(G4_ERR_UNSUPPORTED, "num_sinks must be in [1, 32]");
+  if (p->head_dim != 256 || p->window < 1)
+    return fail(G4_ERR_UNSUPPORTED, "sinks need head_dim 256 and a window");
+  if (p->vision_ids != nullptr || p->document_ids != nullptr)
+    return fail(G4_ERR_UNSUPPORTED, "sinks are not combined with vision or document IDs");
+  return G4_OK;
+}
+
+// [the sinks' dK and dV][the workspace of g4_attn_bwd] in the backward.
+static size_t sinks_bwd_front(const g4_problem& p) { return align256(g4::sinks_part_bytes(p)); }
+
+size_t g4_sinks_workspace_bytes(const g4_problem* p, int32_t num_sinks, int phase) {
+  g_last_error.clear();
+  if (check_sinks(p, num_sinks) != G4_OK) return 0;
+  if (phase == 0) return g4::split_bytes(*p, kSinkTiles);
+  return sinks_bwd_front(*p) + g4_workspace_bytes(p, phase == 2 ? 2 : 1);
+}
+
+static int check_sinks_ws(size_t need, const void* ws, size_t bytes) {
+  if (bytes < need || (need > 0 && ws == nullptr) || ((uintptr_t)ws) % 256) {
+    char buf[128];
+    snprintf(buf, sizeof buf, "%zu bytes at 256 needed, %zu given", need, bytes);
+    return fail(G4_ERR_WORKSPACE, "sink attention workspace: %s", buf);
+  }
+  return G4_OK;
+}
+
+int g4_attn_sinks_fwd(const g4_problem* p, int32_t num_sinks, const void* q, g4_layout ql,
+                      const void* k, g4_layout kl, const void* v, g4_layout vl, void* o,
+                      g4_layout ol, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_sinks(p, num_sinks));
+  G4_TRY(check_fwd_operands(p, q, ql, k, kl, v, vl, o, ol, lse));
+  G4_TRY(check_sinks_ws(g4::split_bytes(*p, kSinkTiles), ws, ws_bytes));
+  return fwd_impl(p, q, ql, k, kl, v, vl, o, ol, lse, ws, ws_bytes, (hipStream_t)stream, num_sinks);
+}
+
+int g4_attn_sinks_bwd(const g4_problem* p, int32_t num_sinks, const void* q, g4_layout ql,
+                      const void* k, g4_layout kl, const void* v, g4_layout vl, const void* o,
+                      g4_layout ol, const void* dout, g4_layout dol, const float* lse,
+                      const float* dlse, void* dq, g4_layout dql, void* dk, g4_layout dkl,
+                      void* dv, g4_layout dvl, void* ws, size_t ws_bytes, void* stream) {
+  g_last_error.clear();
+  G4_TRY(check_sinks(p, num_sinks));
+  const size_t front = sinks_bwd_front(*p);
+  G4_TRY(check_sinks_ws(front + bwd_ws_bytes(*p), ws, ws_bytes));
+  char* const base = (char*)ws + front;
+  // the window's part, with the whole rows' LSE and delta
+  G4_TRY(g4_attn_bwd(p, q, ql, k, kl, v, vl, o, ol, dout, dol, lse, dlse, dq, dql, dk, dkl, dv, dvl,
+                     base, ws_bytes - front, stream));
+  g4::BwdParams a{};
+  fill_bwd(a, p, q, ql, k, kl, v, vl, base);
+  a.dout = (const __bf16*)dout;
+  a.dol = dol;
+  a.lse = lse;
+  a.dq = (__bf16*)dq;
+  a.dql = dql;
+  a.dk = (__bf16*)dk;
+  a.dv = (__bf16*)dv;
+  a.dkl = dkl;
+  a.dvl = dvl;
+  hipError_t e = g4::launch_sinks_bwd(a, num_sinks, (float*)ws, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "backward of the sinks");
   return G4_OK;
 }
 

@@ -58,7 +58,10 @@ constexpr float kRescaleLog2 = 8.0f;
 
 // META: key metadata kinds compiled in (bit 0 vision IDs, bit 1 document IDs).
 // KS: wave groups that share the key tiles, each taking every KS-th one.
-template <int D, int BN, int DSPLIT, int NQG, bool VDOUBLE, int META, int OCC = 1, int KS = 1>
+// SINKS: the first `sinks` keys stay visible behind the window: the tiles that hold
+// them come before the window's, and the tiles between are skipped.
+template <int D, int BN, int DSPLIT, int NQG, bool VDOUBLE, int META, int OCC = 1, int KS = 1,
+          bool SINKS = false>
 struct FwdKernel {
   using C = FwdCfg<D, BN, DSPLIT, NQG, VDOUBLE>;
   static constexpr int kNB = C::kDH / 32;  // 32-wide head-dim blocks per wave
@@ -71,6 +74,7 @@ struct FwdKernel {
   int my_a, my_vid, my_doc;
   bool has_vid, has_doc, has_meta;
   int a0;
+  int sinks, sink_tiles, first_x;  // SINKS: keys, tiles of them, index of this walk's first tile
   const __bf16* kbase;
   const __bf16* vbase;
   int64_t kstride, vstride;
@@ -137,7 +141,8 @@ struct FwdKernel {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = kb0 + jl0 + e;
-          const bool in_w = j >= lo_w;
+          bool in_w = j >= lo_w;
+          if constexpr (SINKS) in_w |= j < sinks;
           const bool causal = in_w & (j <= hi_c);
           const bool vis = has_vid & (my_vid >= 0) & (vk[e] == my_vid) & in_w & (j < sq.lk);
           const bool doc_ok = !has_doc | (dk[e] == my_doc);
@@ -145,6 +150,28 @@ struct FwdKernel {
           sacc[kb][r4 * 4 + e] = ok ? sacc[kb][r4 * 4 + e] : kNegInf;
         }
       }
+  }
+
+  // First key of the walk's tile `it`, whose tiles are t_first, t_first + KS, ...;
+  // with SINKS the tiles 0 .. sink_tiles - 1, then t_first, t_first + 1, ..., of which
+  // the walk takes every KS-th from index first_x on.
+  __device__ __forceinline__ int tile_key(int it, int t_first) const {
+    if constexpr (SINKS) {
+      const int x = first_x + it * KS;
+      return (x < sink_tiles ? x : t_first + x - sink_tiles) * BN;
+    } else {
+      return (t_first + it * KS) * BN;
+    }
+  }
+  // The tiles that hold sinks, for a walk whose window begins at tile t_first.
+  __device__ __forceinline__ void init_sinks(const FwdParams& a, int t_first) {
+    if constexpr (SINKS) {
+      sinks = a.sinks;
+      sink_tiles = min((min(sinks, sq.lk) + BN - 1) / BN, t_first);
+    } else {
+      sinks = sink_tiles = 0;
+    }
+    first_x = 0;
   }
 
   // AHEAD (double-buffered V, no key metadata): K runs two tiles ahead
@@ -155,7 +182,8 @@ struct FwdKernel {
   template <bool AHEAD = false>
   __device__ __forceinline__ void step(int cur, int it, int ntiles, int t_first) {
     static_assert(!AHEAD || (VDOUBLE && META == 0 && KS == 1), "K-ahead steps");
-    const int kb0 = (t_first + it * KS) * BN;
+    const int kb0 = tile_key(it, t_first);
+    const int kb1 = SINKS ? tile_key(it + 1, t_first) : kb0 + KS * BN;  // the next tile
     // This wave's copies of K (and, double-buffered, V) for this tile have
     // landed; the barrier publishes every wave's copies and ends all reads of
     // the buffers refilled below.  (AHEAD: K(it + 1), issued last, may still
@@ -172,11 +200,11 @@ struct FwdKernel {
     }
     barrier_lds();
     if constexpr (AHEAD) {
-      if (it + 1 < ntiles) issue_v(kb0 + BN, cur ^ 1);
+      if (it + 1 < ntiles) issue_v(kb1, cur ^ 1);
     } else if (it + 1 < ntiles) {
-      issue_k(kb0 + KS * BN, cur ^ 1);
-      if (has_meta && wave == 0) issue_meta(*p, sq, kb0 + KS * BN, smem + C::kLdsMeta + (cur ^ 1) * 512, lane, has_vid, has_doc);
-      if constexpr (VDOUBLE) issue_v(kb0 + KS * BN, cur ^ 1);
+      issue_k(kb1, cur ^ 1);
+      if (has_meta && wave == 0) issue_meta(*p, sq, kb1, smem + C::kLdsMeta + (cur ^ 1) * 512, lane, has_vid, has_doc);
+      if constexpr (VDOUBLE) issue_v(kb1, cur ^ 1);
     }
 
     // S^T partial over this wave's head-dim slice.
@@ -232,7 +260,7 @@ struct FwdKernel {
     if constexpr (AHEAD) {
       // every wave is done reading K(it): after the partial exchange's
       // barrier, or with one wave, once its own S chain has its operands
-      if (it + 2 < ntiles) issue_k(kb0 + 2 * BN, cur);
+      if (it + 2 < ntiles) issue_k(SINKS ? tile_key(it + 2, t_first) : kb0 + 2 * BN, cur);
     }
 
     // Mask (only on tiles the mask does not fully admit), then online softmax
@@ -240,7 +268,8 @@ struct FwdKernel {
     // exponent's FMA, and the row maximum is scaled once: rounding is
     // monotonic, so max(s) * log2 e rounds to the maximum of the scaled scores).
     const bool full = !has_doc && (kb0 + BN <= sq.lk) && (kb0 + BN - 1 <= a0) &&
-                      (p->window <= 0 || kb0 > a0 + C::kBM - 1 - p->window);
+                      (p->window <= 0 || kb0 > a0 + C::kBM - 1 - p->window ||
+                       (SINKS && kb0 + BN <= sinks));
     if (!full) {
       __builtin_amdgcn_sched_barrier(0);
       apply_mask(cur, sacc, kb0);
@@ -297,7 +326,7 @@ struct FwdKernel {
     if constexpr (!VDOUBLE) {
       // Single V buffer: every wave must finish its PV reads before refill.
       barrier_lds();
-      if (it + 1 < ntiles) issue_v(kb0 + KS * BN, 0);
+      if (it + 1 < ntiles) issue_v(kb1, 0);
     }
   }
 };
@@ -577,11 +606,12 @@ struct FwdKeyGroups {
 // KS = 2: two groups of waves, each with LDS of its own, take the even and the
 // odd key tiles; their states are combined at the end.
 template <int D, int BN, int DSPLIT, int NQG, bool VDOUBLE, int META, bool FIXUP, int OCC,
-          int KS = 1>
+          int KS = 1, bool SINKS = false>
 __device__ __forceinline__ void fwd_item(const FwdParams& a, char* smem_all, int L,
                                          FixupItem fix = {}) {
-  using K = FwdKernel<D, BN, DSPLIT, NQG, VDOUBLE, META, OCC, KS>;
+  using K = FwdKernel<D, BN, DSPLIT, NQG, VDOUBLE, META, OCC, KS, SINKS>;
   using C = typename K::C;
+  static_assert(!SINKS || (META == 0 && !FIXUP), "sinks without key metadata");
   static_assert(KS == 1 || (KS == 2 && DSPLIT == 1 && VDOUBLE && !FIXUP && META != 3),
                 "key groups");
   K ker;
@@ -649,10 +679,15 @@ __device__ __forceinline__ void fwd_item(const FwdParams& a, char* smem_all, int
   int klo, khi;
   query_tile_key_range(ker.a0, a_last_valid, sq.lk, p.window, span_max, klo, khi);
   int t_first = klo / BN;
+  ker.init_sinks(a, t_first);
   int ntiles = (khi + BN - 1) / BN - t_first;
+  if constexpr (SINKS) ntiles += ker.sink_tiles;
   const int all_tiles = ntiles;
   if constexpr (KS > 1) {  // this group's
-    t_first += kg;
+    if constexpr (SINKS)
+      ker.first_x = kg;
+    else
+      t_first += kg;
     ntiles = max((all_tiles - kg + KS - 1) / KS, 0);
   }
   // ---- document uniformity -------------------------------------------------
@@ -707,9 +742,10 @@ __device__ __forceinline__ void fwd_item(const FwdParams& a, char* smem_all, int
 
   // ---- prologue: tile 0 (issue order K, key metadata, V) -----------------
   if (ntiles > 0) {
-    ker.issue_k(t_first * BN, 0);
-    if (ker.has_meta && ker.wave == 0) issue_meta(p, sq, t_first * BN, ker.smem + C::kLdsMeta, ker.lane, ker.has_vid, ker.has_doc);
-    ker.issue_v(t_first * BN, 0);
+    const int kb = ker.tile_key(0, t_first);
+    ker.issue_k(kb, 0);
+    if (ker.has_meta && ker.wave == 0) issue_meta(p, sq, kb, ker.smem + C::kLdsMeta, ker.lane, ker.has_vid, ker.has_doc);
+    ker.issue_v(kb, 0);
   }
 
 #pragma unroll
@@ -755,7 +791,7 @@ __device__ __forceinline__ void fwd_item(const FwdParams& a, char* smem_all, int
 }
 
 template <int D, int BN, int DSPLIT, int NQG, bool VDOUBLE, int META, bool FIXUP = false,
-          int OCC = 1, int KS = 1>
+          int OCC = 1, int KS = 1, bool SINKS = false>
 __global__ void __launch_bounds__(NQG * DSPLIT * KS * 64, OCC) fwd_kernel(FwdParams a) {
   using C = FwdCfg<D, BN, DSPLIT, NQG, VDOUBLE>;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -782,8 +818,8 @@ __global__ void __launch_bounds__(NQG * DSPLIT * KS * 64, OCC) fwd_kernel(FwdPar
       fwd_item<D, BN, DSPLIT, NQG, VDOUBLE, META, FIXUP, OCC>(a, smem_raw, 0, it);
     });
   } else {
-    fwd_item<D, BN, DSPLIT, NQG, VDOUBLE, META, FIXUP, OCC, KS>(a, smem_raw,
-                                                                FwdItem::of_block(a));
+    fwd_item<D, BN, DSPLIT, NQG, VDOUBLE, META, FIXUP, OCC, KS, SINKS>(a, smem_raw,
+                                                                       FwdItem::of_block(a));
   }
 }
 
@@ -801,12 +837,12 @@ __global__ void __launch_bounds__(NQG * DSPLIT * KS * 64, OCC) fwd_kernel(FwdPar
 // O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c.
 // ===========================================================================
 
-template <int D>
-using SplitKernel = FwdKernel<D, 32, D / 256, 1, true, 0, (D == 256 ? 2 : 1)>;
+template <int D, bool SINKS = false>
+using SplitKernel = FwdKernel<D, 32, D / 256, 1, true, 0, (D == 256 ? 2 : 1), 1, SINKS>;
 
-template <int D>
+template <int D, bool SINKS = false>
 __global__ void __launch_bounds__(D / 4, (D == 256 ? 2 : 1)) fwd_split_kernel(FwdParams a) {
-  using K = SplitKernel<D>;
+  using K = SplitKernel<D, SINKS>;
   using C = typename K::C;
   constexpr int BN = 32;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -846,9 +882,12 @@ __global__ void __launch_bounds__(D / 4, (D == 256 ? 2 : 1)) fwd_split_kernel(Fw
   int klo, khi;
   query_tile_key_range(off, off + lq - 1, sq.lk, p.window, -1, klo, khi);
   const int per = a.split_keys / BN;
-  const int t_first = klo / BN + c * per;
-  const int t_end = min((khi + BN - 1) / BN, t_first + per);
-  const int ntiles = khi > klo ? max(t_end - t_first, 0) : 0;
+  ker.init_sinks(a, klo / BN);
+  ker.first_x = c * per;
+  const int t_first = SINKS ? klo / BN : klo / BN + c * per;
+  const int t_end = SINKS ? min((khi + BN - 1) / BN - t_first + ker.sink_tiles, (c + 1) * per)
+                          : min((khi + BN - 1) / BN, t_first + per);
+  const int ntiles = khi > klo ? max(t_end - (SINKS ? ker.first_x : t_first), 0) : 0;
 
   ker.kbase = a.k + tok_off(sq, s, sq.ktok, 0, a.kl) + (int64_t)kvh * a.kl.head_stride;
   ker.vbase = a.v + tok_off(sq, s, sq.ktok, 0, a.vl) + (int64_t)kvh * a.vl.head_stride;
@@ -868,9 +907,9 @@ __global__ void __launch_bounds__(D / 4, (D == 256 ? 2 : 1)) fwd_split_kernel(Fw
     }
   }
   if (ntiles > 0) {
-    ker.issue_k(t_first * BN, 0);
-    ker.issue_v(t_first * BN, 0);
-    if (ntiles > 1) ker.issue_k((t_first + 1) * BN, 1);
+    ker.issue_k(ker.tile_key(0, t_first), 0);
+    ker.issue_v(ker.tile_key(0, t_first), 0);
+    if (ntiles > 1) ker.issue_k(ker.tile_key(1, t_first), 1);
   }
 #pragma unroll
   for (int b = 0; b < K::kNB; ++b) ker.o_acc[b] = f32x16{};
@@ -972,19 +1011,19 @@ __global__ void __launch_bounds__(256) merge_split_kernel(FwdParams a) {
     a.lse[lse_off(p, sq, s, qh, qi)] = l > 0.f ? (mx + fast_log2(l)) * kLn2 : kNegInf;
 }
 
-template <int D>
+template <int D, bool SINKS = false>
 static hipError_t launch_fwd_split(const FwdParams& a, hipStream_t stream) {
   using C = typename SplitKernel<D>::C;
   static_assert(C::kNT == D / 4, "one wave per 256 of the head dim");
   static LdsAttr attr;
-  hipError_t e = attr.ensure((const void*)fwd_split_kernel<D>, C::kLdsBytes);
+  hipError_t e = attr.ensure((const void*)fwd_split_kernel<D, SINKS>, C::kLdsBytes);
   if (e != hipSuccess) return e;
   const int64_t groups = (int64_t)a.num_seqs * a.p.num_kv_heads;
   const int64_t rows = (int64_t)(a.p.num_q_heads / a.p.num_kv_heads) * a.p.seqlen_q;
   const int64_t items = groups * a.split_chunks;
   if (items <= 0) return hipSuccess;
-  hipLaunchKernelGGL(fwd_split_kernel<D>, dim3((unsigned)items), dim3(C::kNT), C::kLdsBytes,
-                     stream, a);
+  hipLaunchKernelGGL((fwd_split_kernel<D, SINKS>), dim3((unsigned)items), dim3(C::kNT),
+                     C::kLdsBytes, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(merge_split_kernel<D>, dim3((unsigned)(groups * rows)), dim3(256), 0, stream,
@@ -2161,10 +2200,10 @@ static bool use_fwd_groups(const g4_problem& p, int64_t nblocks) {
   return nblocks > 0 && nblocks <= kCus && keys > 256;
 }
 
-template <int META>
+template <int META, bool SINKS = false>
 static hipError_t launch_fwd_groups(const FwdParams& a, int64_t nblocks, hipStream_t stream) {
   using C = FwdCfg<256, 32, 1, 4, true>;
-  const auto kern = fwd_kernel<256, 32, 1, 4, true, META, false, 1, 2>;
+  const auto kern = fwd_kernel<256, 32, 1, 4, true, META, false, 1, 2, SINKS>;
   static LdsAttr attr;
   hipError_t e = attr.ensure((const void*)kern, FwdKeyGroups<C>::kLdsBytes);
   if (e != hipSuccess) return e;
@@ -2173,11 +2212,30 @@ static hipError_t launch_fwd_groups(const FwdParams& a, int64_t nblocks, hipStre
   return hipGetLastError();
 }
 
+// Head dim 256 with a window and sinks: the text kernels with the sinks' tiles first.
+static hipError_t launch_fwd_sinks(const FwdParams& a, hipStream_t stream) {
+  if (a.p.head_dim != 256 || meta_kind(a.p) != 0 || a.p.window <= 0) return hipErrorInvalidValue;
+  if (a.split_chunks > 0) return launch_fwd_split<256, true>(a, stream);
+  using C = FwdCfg<256, 32, 1, 4, true>;
+  FwdParams b = a;
+  b.doc_pass = 0;
+  const int64_t n = fwd_grid(&b, C::kBM, true);
+  if (n <= 0) return hipSuccess;
+  if (use_fwd_groups(a.p, n)) return launch_fwd_groups<0, true>(b, n, stream);
+  const auto kern = fwd_kernel<256, 32, 1, 4, true, 0, false, 2, 1, true>;
+  static LdsAttr attr;
+  hipError_t e = attr.ensure((const void*)kern, C::kLdsBytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)n), dim3(C::kNT), C::kLdsBytes, stream, b);
+  return hipGetLastError();
+}
+
 __global__ void clear_list_kernel(unsigned* n) {
   if (threadIdx.x == 0) *n = 0u;
 }
 
 hipError_t launch_fwd(const FwdParams& a, hipStream_t stream) {
+  if (a.sinks > 0) return launch_fwd_sinks(a, stream);
   if (a.split_slots > 0)
     return a.p.cu_seqlens_q != nullptr && a.num_seqs <= 64 ? launch_fwd_decode<512, true>(a, stream)
                                                            : launch_fwd_decode<512, false>(a, stream);

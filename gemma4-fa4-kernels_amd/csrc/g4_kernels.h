@@ -53,6 +53,9 @@ struct FwdParams {
   // 1 unless `part` holds the chunks' partial rows).
   int kv_chunks;
   float* part;
+  // Head dim 256 with a window, without key metadata: the first `sinks` keys of a
+  // sequence stay visible (0: the plain window).
+  int sinks;
 };
 
 // Query (0..31, within its 32-query row) at position p of a dS tile's key row:
@@ -213,13 +216,14 @@ int ds_stripes(const g4_problem& p, DsStripe* out, int max_out);
 size_t acc_bytes(const g4_problem& p);
 // Split-key forward: the number of key chunks per (sequence, KV head), 0 when
 // the problem takes the regular forward; *keys receives the keys per chunk.
-int split_chunks(const g4_problem& p, int* keys);
+// extra_tiles: key tiles walked beside the window's (the sinks').
+int split_chunks(const g4_problem& p, int* keys, int extra_tiles = 0);
 // Wide head-dim 512 forward: key chunks per query tile (1: not split) and the
 // workspace bytes of their partial rows.
 int wide_chunks(const g4_problem& p);
 size_t wide_split_bytes(const g4_problem& p);
 // Workspace bytes of its partial rows (0 when not split).
-size_t split_bytes(const g4_problem& p);
+size_t split_bytes(const g4_problem& p, int extra_tiles = 0);
 // Decode with equal parts: their number (0 when the problem takes the chunks
 // of split_chunks) and the workspace bytes of their slots of partial rows.
 int decode_parts(const g4_problem& p);
@@ -242,6 +246,14 @@ hipError_t launch_fwd(const FwdParams& a, hipStream_t stream);
 hipError_t launch_bwd_delta(const BwdParams& a, hipStream_t stream);
 hipError_t launch_bwd_dkdv(const BwdParams& a, hipStream_t stream);
 hipError_t launch_bwd_dq(const BwdParams& a, hipStream_t stream);
+// The sinks' part of the backward at head dim 256 with a window (g4_sinks.hip).
+struct SinkParams {
+  BwdParams b;
+  int sinks, chunk;  // keys; queries of a workgroup
+  float* part;       // the chunks' dK and dV
+};
+size_t sinks_part_bytes(const g4_problem& p);
+hipError_t launch_sinks_bwd(const BwdParams& b, int sinks, float* part, hipStream_t stream);
 hipError_t launch_mask(const g4_problem& p, uint8_t* out, const int* span_lo, const int* span_hi,
                        hipStream_t stream);
 hipError_t launch_ranges(const g4_problem& p, int direction, int row_tile, int32_t* out,

@@ -1,0 +1,350 @@
+// Backward of the sinks: the keys that a sliding window leaves visible at the
+// beginning of each sequence.
+//
+// The window's part of the gradients comes from the text kernels: with the LSE
+// and delta of the whole row, P = exp(S - LSE) and dS = P (dP - delta) of a pair
+// do not depend on which other pairs the row has.  What is left, for sequences
+// longer than the window:
+//   dQ += dS K over the sinks behind the window (added to the stored rows), and
+//   dK, dV of the sinks, over every query of the sequence (written anew, so that
+//   each is one fp32 sum rounded once).
+// A workgroup takes a chunk of a sequence's queries and one KV head; its waves
+// take 32 rows of one query head at a time: S = Q K^T and dP = dO V^T with keys
+// along lanes feed dV^T += dO^T P and dK^T += Q^T dS from registers, the same
+// products with the operands exchanged (S^T, dP^T: queries along lanes) feed
+// dQ^T = K^T dS^T.  The chunk's dK and dV go to the workspace and a second launch
+// adds the chunks in order (no atomics).  Bound by HBM: Q, dO and dQ are read and
+// dQ is written once more, 4 x 512 bytes a row.
+#include "g4_kernels.h"
+
+namespace g4 {
+
+namespace {
+
+constexpr int kSinkKeys = G4_MAX_SINKS;  // one 32-key block
+constexpr int D = 256;
+constexpr int kNC = D / 16;  // 16-deep steps of S and dP
+constexpr int kNB = D / 32;  // 32-wide blocks of the head dim
+constexpr int kWaves = 4;
+constexpr int kRowsBytes = 32 * D * 2;            // a tile of Q or dO
+constexpr int kWaveBytes = 2 * kRowsBytes;        // = 32 fp32 rows of D
+constexpr int kLdsK = kWaves * kWaveBytes;
+constexpr int kLdsStat = kLdsK + kRowsBytes;      // [wave][LSE x 32 | delta x 32] fp32
+constexpr int kLdsBytes = kLdsStat + kWaves * 256;
+static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
+static_assert(kWaveBytes == 32 * D * 4, "the sums of a wave fit its tiles");
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Chunks of sequence s: none where the window reaches every key.
+__device__ __forceinline__ int sink_chunks(const SinkParams& a, int s) {
+  const Seq q = resolve_seq(a.b.p, s);
+  return q.lk > a.b.p.window && q.lq > 0 ? (q.lq + a.chunk - 1) / a.chunk : 0;
+}
+
+// Sequence and chunk of slot x (slots number the chunks of all sequences);
+// false past the last.  Every lane of the wave calls it.
+__device__ __forceinline__ bool sink_slot(const SinkParams& a, int x, int& s, int& c) {
+  const int lane = __lane_id();
+  int base = 0;
+  for (int s0 = 0; s0 < a.b.p.num_seqs; s0 += 64) {
+    const int n = s0 + lane < a.b.p.num_seqs ? sink_chunks(a, s0 + lane) : 0;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    if (x < base + total) {
+      const int k = __popcll(__ballot(base + incl <= x));
+      s = __builtin_amdgcn_readfirstlane(s0 + k);
+      c = __builtin_amdgcn_readfirstlane(x - base - __shfl(incl - n, k, 64));
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+// Slots before sequence s.
+__device__ __forceinline__ int sink_slots_before(const SinkParams& a, int s) {
+  int n = 0;
+  for (int j = __lane_id(); j < s; j += 64) n += sink_chunks(a, j);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  return __builtin_amdgcn_readfirstlane(n);
+}
+
+// x = rows . keys^T (keys along lanes) and, with BOTH, y = keys . rows^T; the keys'
+// fragments from `keys`, a tile in LDS (K) or registers (V).
+template <int CP, class RR>
+__device__ __forceinline__ bf16x8 sink_fragment(const RR& rrd, const char G4_LDS* t) {
+  return rrd.template read<0, 0, CP>(t);
+}
+template <int CP, class RR>
+__device__ __forceinline__ bf16x8 sink_fragment(const RR&, const bf16x8 (&f)[kNC]) {
+  return f[CP];
+}
+template <bool BOTH, int CP, class RR, class Keys>
+__device__ __forceinline__ void sink_products(const RR& rrd, const char G4_LDS* rows,
+                                              const Keys& keys, f32x16& x, f32x16& y) {
+  if constexpr (CP < kNC) {
+    const bf16x8 f = rrd.template read<0, 0, CP>(rows), g = sink_fragment<CP>(rrd, keys);
+    x = mfma32(f, g, x);
+    if constexpr (BOTH) y = mfma32(g, f, y);
+    sink_products<BOTH, CP + 1>(rrd, rows, keys, x, y);
+  }
+}
+
+// Byte of the 16-byte chunk c of fp32 row r in a wave's area (D * 4 bytes a row).
+__device__ __forceinline__ int sum_off(int r, int c) { return r * D * 4 + (c ^ r) * 16; }
+
+template <int B, class TR>
+__device__ __forceinline__ void sink_dq(const TR& trd, const char G4_LDS* kt,
+                                        const bf16x8 (&ds)[2], char G4_LDS* stage, int l32,
+                                        int h32) {
+  if constexpr (B < kNB) {
+    f32x16 acc = {};
+    acc = mfma32(trd.template read<0, 0, B>(kt), ds[0], acc);
+    acc = mfma32(trd.template read<16, 0, B>(kt), ds[1], acc);
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4)
+      *(f32x4 G4_LDS*)(stage + sum_off(l32, 8 * B + 2 * r4 + h32)) =
+          f32x4{acc[4 * r4], acc[4 * r4 + 1], acc[4 * r4 + 2], acc[4 * r4 + 3]};
+    sink_dq<B + 1>(trd, kt, ds, stage, l32, h32);
+  }
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  char G4_LDS* const smem = (char G4_LDS*)smem_raw;
+  const BwdParams& a = sp.b;
+  const g4_problem& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h32 = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.num_kv_heads, slot = blockIdx.x / p.num_kv_heads;
+  int s, chunk;
+  if (!sink_slot(sp, slot, s, chunk)) return;
+  const Seq sq = resolve_seq(p, s);
+  const int off = sq.lk - sq.lq;
+  const int grp = p.num_q_heads / p.num_kv_heads;
+  const int sinks = min(sp.sinks, sq.lk);
+
+  // ---- the sinks' K and V: rows past them as zeros -----------------------------
+  const __bf16* kbase = a.k + tok_off(sq, s, sq.ktok, 0, a.kl) + (int64_t)kvh * a.kl.head_stride;
+  const __bf16* vbase = a.v + tok_off(sq, s, sq.ktok, 0, a.vl) + (int64_t)kvh * a.vl.head_stride;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = i * 256 + tid, r = x / 32, c = x % 32;
+    const bf16x8 y = r < sinks ? ld_global16(kbase + r * a.kl.token_stride + c * 8) : bf16x8{};
+    *(bf16x8 G4_LDS*)(smem + kLdsK + (r * 32 + swz_slot(r, c)) * 16) = y;
+  }
+  bf16x8 vf[kNC];
+  {
+    const __bf16* vrow = vbase + min(l32, sinks - 1) * a.vl.token_stride + h32 * 8;
+#pragma unroll
+    for (int c = 0; c < kNC; ++c) {
+      const bf16x8 y = ld_global16(vrow + c * 16);
+      vf[c] = l32 < sinks ? y : bf16x8{};
+    }
+  }
+  barrier_lds();
+  RowReader<32> rrd;
+  TrReader<32> trd;
+  rrd.init(lane);
+  trd.init(lane);
+  const char G4_LDS* const kt = smem + kLdsK;
+
+  // ---- the chunk's rows -----------------------------------------------------------
+  char G4_LDS* const qt = smem + wave * kWaveBytes;
+  char G4_LDS* const dot = qt + kRowsBytes;
+  float G4_LDS* const stat = (float G4_LDS*)(smem + kLdsStat + wave * 256);
+  TileCopier<32, 32, 1> qcp, docp;
+  qcp.init(a.ql.token_stride, 0, lane);
+  docp.init(a.dol.token_stride, 0, lane);
+  f32x16 dk[kNB], dv[kNB];
+#pragma unroll
+  for (int b = 0; b < kNB; ++b) dk[b] = dv[b] = f32x16{};
+  const int i_end = min((chunk + 1) * sp.chunk, sq.lq);
+  const int tiles = (i_end - chunk * sp.chunk + 31) / 32;
+  for (int t = wave; t < tiles * grp; t += kWaves) {
+    const int i0 = chunk * sp.chunk + t / grp * 32, qh = kvh * grp + t % grp;
+    const int nrows = min(i_end - i0, 32);
+    const __bf16* qrow = a.q + tok_off(sq, s, sq.qtok, i0, a.ql) + (int64_t)qh * a.ql.head_stride;
+    const __bf16* dorow =
+        a.dout + tok_off(sq, s, sq.qtok, i0, a.dol) + (int64_t)qh * a.dol.head_stride;
+    wait_lds();  // the previous tile's reads
+    if (nrows == 32) {
+      qcp.issue(qrow, qt);
+      docp.issue(dorow, dot);
+    } else {
+      qcp.issue_clamped(qrow, 0, nrows, qt);
+      docp.issue_clamped(dorow, 0, nrows, dot);
+    }
+    {
+      // LSE and delta of the rows; a row that sees nothing has no weights
+      const int64_t at = lse_off(p, sq, s, qh, i0 + min(l32, nrows - 1));
+      const int64_t tok = (int64_t)qh * q_stream_tokens_dev(p) + sq.qtok + i0 + min(l32, nrows - 1);
+      const float lse = a.lse[at];
+      const float x = h32 ? a.delta[tok] : lse == kNegInf ? -kNegInf : lse * kLog2e;
+      stat[lane] = x;
+    }
+    vm_wait<0>();
+    wait_lds();
+
+    const int a0 = i0 + off;
+    const bool far = a0 + nrows - 1 >= p.window;  // a row with sinks behind its window
+    f32x16 sc = {}, st = {}, dp = {}, dpt = {};
+    if (far) {
+      sink_products<true, 0>(rrd, qt, kt, sc, st);
+      sink_products<true, 0>(rrd, dot, vf, dp, dpt);
+    } else {
+      sink_products<false, 0>(rrd, qt, kt, sc, st);
+      sink_products<false, 0>(rrd, dot, vf, dp, dpt);
+    }
+    bf16x8 pb[2], dsb[2], dst[2];
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const f32x4 lse = *(const f32x4 G4_LDS*)(stat + 8 * r4 + 4 * h32);
+      const f32x4 dl = *(const f32x4 G4_LDS*)(stat + 32 + 8 * r4 + 4 * h32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * r4 + e, row = 8 * r4 + 4 * h32 + e;
+        const bool ok = (l32 < sinks) & (l32 <= a0 + row) & (row < nrows);
+        const float pr = ok ? fast_exp2(__builtin_fmaf(sc[r], kLog2e, -lse[e])) : 0.f;
+        const float ds = ok ? pr * (dp[r] - dl[e]) : 0.f;
+        pb[r / 8][r % 8] = (__bf16)pr;
+        dsb[r / 8][r % 8] = (__bf16)ds;
+      }
+    }
+    if (far) {
+      const float lse = stat[l32], dl = stat[32 + l32];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = 8 * (r / 4) + 4 * h32 + r % 4;
+        const bool ok = (key < sinks) & (key <= a0 + l32 - p.window);
+        const float pr = ok ? fast_exp2(__builtin_fmaf(st[r], kLog2e, -lse)) : 0.f;
+        dst[r / 8][r % 8] = (__bf16)(ok ? pr * (dpt[r] - dl) : 0.f);
+      }
+    }
+    acc_steps<kNB>(trd, dot, pb, dv);
+    acc_steps<kNB>(trd, qt, dsb, dk);
+    if (far) {
+      // dQ's rows in fp32 over the tiles just used, then whole rows added to memory.
+      // (The lane passes through an empty asm: the swizzled offsets derived from it are
+      // formed here, not held in registers across the loop.)
+      wait_lds();
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      const int l32 = ln & 31, h32 = ln >> 5;
+      sink_dq<0>(trd, kt, dst, qt, l32, h32);
+      __bf16* const dqrow = a.dq + tok_off(sq, s, sq.qtok, i0, a.dql) +
+                            (int64_t)qh * a.dql.head_stride + l32 * 8;
+      wait_lds();
+#pragma unroll 1
+      for (int j = 0; j < 16; j += 8) {
+        bf16x8 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          y[i] = ld_global16(dqrow +
+                             (int64_t)min(2 * (j + i) + h32, nrows - 1) * a.dql.token_stride);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = 2 * (j + i) + h32;
+          const f32x4 u = *(const f32x4 G4_LDS*)(qt + sum_off(row, 2 * l32));
+          const f32x4 v = *(const f32x4 G4_LDS*)(qt + sum_off(row, 2 * l32 + 1));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[i][e] = (__bf16)((float)y[i][e] + u[e]);
+            y[i][4 + e] = (__bf16)((float)y[i][4 + e] + v[e]);
+          }
+          // (a row before the window's reach gets zeros added: its bits stay)
+          if (row < nrows) *(bf16x8*)(dqrow + (int64_t)row * a.dql.token_stride) = y[i];
+        }
+      }
+    }
+  }
+
+  // ---- the waves' sums, key by key --------------------------------------------------
+  float* const part = sp.part + ((int64_t)slot * p.num_kv_heads + kvh) * 2 * kSinkKeys * D;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    barrier_lds();
+#pragma unroll
+    for (int b = 0; b < kNB; ++b)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x16& x = which ? dv[b] : dk[b];
+        *(f32x4 G4_LDS*)(qt + sum_off(l32, 8 * b + 2 * r4 + h32)) =
+            f32x4{x[4 * r4], x[4 * r4 + 1], x[4 * r4 + 2], x[4 * r4 + 3]};
+      }
+    barrier_lds();
+    for (int r = wave; r < sinks; r += kWaves) {
+      f32x4 x = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        x += *(const f32x4 G4_LDS*)(smem + w * kWaveBytes + sum_off(r, lane));
+      *(f32x4*)(part + (which * kSinkKeys + r) * D + 4 * lane) = x;
+    }
+  }
+}
+
+// dK and dV of the sinks from the chunks' sums.  One wave per (sequence, KV head,
+// K or V, sink).
+__global__ void __launch_bounds__(64) sinks_sum_kernel(SinkParams sp) {
+  const BwdParams& a = sp.b;
+  const g4_problem& p = a.p;
+  const int kvh = blockIdx.x % p.num_kv_heads, s = blockIdx.x / p.num_kv_heads;
+  const int r = blockIdx.y % sp.sinks, which = blockIdx.y / sp.sinks;
+  const int n = sink_chunks(sp, s);
+  const Seq sq = resolve_seq(p, s);
+  if (n == 0 || r >= sq.lk) return;
+  const int first = sink_slots_before(sp, s);
+  const int lane = threadIdx.x;
+  const int64_t pitch = (int64_t)p.num_kv_heads * 2 * kSinkKeys * D;
+  const float* src = sp.part + (int64_t)first * pitch +
+                     ((int64_t)kvh * 2 * kSinkKeys + which * kSinkKeys + r) * D + 4 * lane;
+  f32x4 x = {};
+#pragma unroll 8
+  for (int c = 0; c < n; ++c) x += *(const f32x4*)(src + c * pitch);
+  const g4_layout& l = which ? a.dvl : a.dkl;
+  *(bf16x4*)((which ? a.dv : a.dk) + tok_off(sq, s, sq.ktok, r, l) + (int64_t)kvh * l.head_stride +
+             4 * lane) = bf16x4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+}
+
+// Queries of a chunk: about two workgroups per CU in all.
+static int sink_chunk(const g4_problem& p) {
+  const int64_t rows = q_stream_tokens(p) * p.num_kv_heads;
+  return (int)((rows / 512 + 31) / 32 * 32) + (rows < 512 ? 32 : 0);
+}
+
+// Chunks at most: sequences that a window does not cover have more keys than it.
+static int64_t sink_slots(const g4_problem& p) {
+  const int64_t longer = std::min<int64_t>(p.num_seqs, k_stream_tokens(p) / (p.window + 1));
+  return q_stream_tokens(p) / sink_chunk(p) + longer;
+}
+
+size_t sinks_part_bytes(const g4_problem& p) {
+  return (size_t)sink_slots(p) * p.num_kv_heads * 2 * kSinkKeys * D * 4;
+}
+
+hipError_t launch_sinks_bwd(const BwdParams& b, int sinks, float* part, hipStream_t stream) {
+  SinkParams a{b, sinks, sink_chunk(b.p), part};
+  const int64_t blocks = sink_slots(b.p) * b.p.num_kv_heads;
+  if (blocks <= 0) return hipSuccess;  // no sequence is longer than the window
+  static LdsAttr attr;
+  hipError_t e = attr.ensure((const void*)sinks_bwd_kernel, kLdsBytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(sinks_bwd_kernel, dim3((unsigned)blocks), dim3(256), kLdsBytes, stream, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(sinks_sum_kernel, dim3((unsigned)(b.p.num_seqs * b.p.num_kv_heads),
+                                            (unsigned)(2 * sinks)),
+                     dim3(64), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace g4

@@ -12,6 +12,7 @@ from .attention import (
     fa4_global_varlen_forward,
     fa4_global_varlen_forward_only,
     fa4_local_forward,
+    fa4_local_sinks_varlen_forward,
     fa4_local_text_forward,
     fa4_local_varlen_forward,
     pin_backward_ds_budget,
@@ -67,6 +68,7 @@ __all__ = [
     "fa4_local_forward",
     "fa4_local_text_forward",
     "fa4_local_varlen_forward",
+    "fa4_local_sinks_varlen_forward",
     "fa4_global_text_forward",
     "fa4_global_forward_only",
     "fa4_global_varlen_forward",

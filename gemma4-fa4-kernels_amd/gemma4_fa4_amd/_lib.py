@@ -52,6 +52,9 @@ EXPORTED_SYMBOLS = (
     "g4_pages_release",
     "g4_pages_compact",
     "g4_pages_copy",
+    "g4_sinks_workspace_bytes",
+    "g4_attn_sinks_fwd",
+    "g4_attn_sinks_bwd",
 )
 
 
@@ -183,6 +186,14 @@ _SIGNATURES = {
     "g4_pages_release": (ctypes.c_int, [_TABLE, _P, _I32, _I32, _P, _I32, _I32, _P]),
     "g4_pages_compact": (ctypes.c_int, [_TABLE, _P, _I32, _P, _P, _P, _SZ, _P]),
     "g4_pages_copy": (ctypes.c_int, [_CACHE, _P, _P, _I32, _P]),
+    "g4_sinks_workspace_bytes": (ctypes.c_size_t, [_PROB, _I32, ctypes.c_int]),
+    "g4_attn_sinks_fwd": (
+        ctypes.c_int, [_PROB, _I32, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _SZ, _P]),
+    "g4_attn_sinks_bwd": (
+        ctypes.c_int,
+        [_PROB, _I32, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _L, _P, _L, _P, _L, _P,
+         _SZ, _P],
+    ),
 }
 
 _lock = threading.Lock()

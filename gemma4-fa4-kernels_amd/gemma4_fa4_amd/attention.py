@@ -38,6 +38,7 @@ _GLOBAL_NATIVE_BACKWARD_MAX_SEQLEN = _LOCAL_MODEL_MAX_SEQLEN
 _GLOBAL_BACKWARD_RESERVE_BYTES = 2 * 1024**3
 _METADATA_WORKSPACE_MAX_BYTES = 2 * 1024**3
 _TARGET_ARCH = "gfx950"
+_MAX_SINKS = 32
 
 
 # ---------------------------------------------------------------------------
@@ -553,6 +554,8 @@ class _Plan:
     spare_bytes: int | None = None
     # The free-HBM reading of the forward's checks, if they took one.
     free_bytes: int | None = None
+    # First tokens of each sequence that stay visible behind the window (local text).
+    num_sinks: int = 0
     # Cumulative-array checks still to run before the first launch.
     pending: _CumulativeCheck | None = field(default=None, repr=False, compare=False)
     # Workspace sizes already asked of the library, by (phase, ds_budget): the
@@ -602,7 +605,10 @@ class _Plan:
         lib = _lib.load()
         if prob is None:
             prob = self.problem()
-        nbytes = int(lib.g4_workspace_bytes(ctypes.byref(prob), phase))
+        if self.num_sinks:
+            nbytes = int(lib.g4_sinks_workspace_bytes(ctypes.byref(prob), self.num_sinks, phase))
+        else:
+            nbytes = int(lib.g4_workspace_bytes(ctypes.byref(prob), phase))
         if nbytes == 0 and lib.g4_last_error():
             _lib.check(_lib.G4_ERR_INVALID)
         self._ws_sizes[key] = nbytes
@@ -641,6 +647,10 @@ class _Plan:
         # takes NULL for a zero-byte workspace, so none is allocated.
         return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
 
+    def _sinks(self) -> tuple[int, ...]:
+        """The argument that the sink entry points take after the problem."""
+        return (self.num_sinks,) if self.num_sinks else ()
+
     def forward(self, q, k, v):
         try:
             lib = _lib.load()
@@ -654,7 +664,7 @@ class _Plan:
         with _lib.device_scope(q.device):
             stream = _lib.raw_stream(q.device)
             args = (
-                ctypes.byref(prob),
+                ctypes.byref(prob), *self._sinks(),
                 q.data_ptr(), _layout(q, self.packed),
                 k.data_ptr(), _layout(k, self.packed),
                 v.data_ptr(), _layout(v, self.packed),
@@ -662,7 +672,7 @@ class _Plan:
                 lse.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes, stream,
             )
             self._settle()
-            rc = lib.g4_attn_fwd(*args)
+            rc = (lib.g4_attn_sinks_fwd if self.num_sinks else lib.g4_attn_fwd)(*args)
         _lib.check(rc)
         return out, lse
 
@@ -679,8 +689,8 @@ class _Plan:
         ws = self._workspace(1, q.device, prob)
         with _lib.device_scope(q.device):
             stream = _lib.raw_stream(q.device)
-            rc = lib.g4_attn_bwd(
-                ctypes.byref(prob),
+            rc = (lib.g4_attn_sinks_bwd if self.num_sinks else lib.g4_attn_bwd)(
+                ctypes.byref(prob), *self._sinks(),
                 q.data_ptr(), _layout(q, self.packed),
                 k.data_ptr(), _layout(k, self.packed),
                 v.data_ptr(), _layout(v, self.packed),
@@ -1047,6 +1057,47 @@ def fa4_local_varlen_forward(
             free = _preflight_metadata_workspace(plan, q.device)
         if _requires_backward(q, k, v):
             _fit_local_backward(plan, q, k, v, free)
+        return plan
+
+    return _run_checked(q, k, v, check, prepare)
+
+
+def fa4_local_sinks_varlen_forward(
+    q,
+    k,
+    v,
+    cu_seqlens_q,
+    cu_seqlens_k,
+    *,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    num_sinks: int,
+    spec: AttentionLayerSpec = SLIDING_ATTENTION,
+):
+    """Packed local text attention whose sequences' first tokens stay visible, autograd-capable.
+
+    As ``fa4_local_varlen_forward`` without metadata, with the mask ``k <= q`` and
+    (``k > q - 1024`` or ``k < num_sinks``): the first ``num_sinks`` (up to 32) tokens of
+    each K segment, sinks, keep their place in every softmax after the window has
+    passed them, so that a model trained so can be served from a cache that keeps only
+    them and the window (``paged_cache_attention``, ``release_pages``).  The reference has
+    no counterpart.  One forward launch (two for a few queries); the backward is the local
+    one with the whole rows' LSE and delta, and a pass over the sinks.  As with the other
+    adapters, a NaN or an infinity in V can reach rows that exclude its key.
+    """
+    if not _is_python_int(num_sinks):
+        raise TypeError("num_sinks must be a Python integer")
+    if not 0 <= num_sinks <= _MAX_SINKS:
+        raise UnsupportedMI355XPath(f"num_sinks must be in [0, {_MAX_SINKS}]")
+    check = _validate_local_varlen(
+        q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, spec
+    )
+
+    def prepare():
+        plan = _packed_plan(q, k, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, spec)
+        plan.num_sinks = num_sinks
+        if _requires_backward(q, k, v):
+            _fit_local_backward(plan, q, k, v)
         return plan
 
     return _run_checked(q, k, v, check, prepare)

@@ -28,6 +28,7 @@ import torch
 from . import _lib
 from ._lib import G4CacheAttn, G4Layout, G4PagedCache, G4PageTable
 from .attention import (
+    _MAX_SINKS,
     _check_real_operands,
     _empty_as,
     _is_python_int,
@@ -190,7 +191,6 @@ def paged_cache_gather(
     return k, v
 
 
-MAX_SINKS = 32  # first tokens that a windowed layer may keep visible
 _MAX_LENGTH = 1 << 30
 
 
@@ -237,8 +237,8 @@ def paged_cache_attention(
         raise ValueError("max_seqlen_q and max_seqlen_k must be in [1, 2^30]")
     if sliding_window is not None and sliding_window < 1:
         raise ValueError("sliding_window must be positive")
-    if not 0 <= num_sinks <= MAX_SINKS:
-        raise UnsupportedMI355XPath("num_sinks must be in [0, 32]")
+    if not 0 <= num_sinks <= _MAX_SINKS:
+        raise UnsupportedMI355XPath(f"num_sinks must be in [0, {_MAX_SINKS}]")
     if sliding_window is None and num_sinks:
         raise ValueError("num_sinks needs a sliding_window")
     if head_dim == 512 and sliding_window is not None:

@@ -460,6 +460,35 @@ int g4_pages_compact(const g4_page_table* table, int32_t* ref_counts, int32_t nu
 int g4_pages_copy(const g4_paged_cache* cache, const int32_t* src, const int32_t* dst,
                   int32_t count, void* stream);
 
+/*
+ * Attention with a sliding window and sinks: g4_attn_fwd / g4_attn_bwd of a
+ * head-dim 256 problem with a window and without key metadata, whose first
+ * num_sinks (1..G4_MAX_SINKS) tokens of each sequence stay visible:
+ * allowed(q, k) = k <= q AND (k > q - window OR k < num_sinks).
+ * g4_sinks_workspace_bytes: phase 0 the forward, 1 the backward, 2 the backward
+ * with the larger workspace of g4_workspace_bytes.
+ */
+size_t g4_sinks_workspace_bytes(const g4_problem* p, int32_t num_sinks, int phase);
+
+int g4_attn_sinks_fwd(const g4_problem* p, int32_t num_sinks,
+                      const void* q, g4_layout q_layout,
+                      const void* k, g4_layout k_layout,
+                      const void* v, g4_layout v_layout,
+                      void* o, g4_layout o_layout, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+int g4_attn_sinks_bwd(const g4_problem* p, int32_t num_sinks,
+                      const void* q, g4_layout q_layout,
+                      const void* k, g4_layout k_layout,
+                      const void* v, g4_layout v_layout,
+                      const void* o, g4_layout o_layout,
+                      const void* dout, g4_layout do_layout,
+                      const float* lse, const float* dlse,
+                      void* dq, g4_layout dq_layout,
+                      void* dk, g4_layout dk_layout,
+                      void* dv, g4_layout dv_layout,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
