@@ -1129,8 +1129,10 @@ static int check_sinks(const g4_problem* p, int32_t num_sinks) {
   return G4_OK;
 }
 
-// [the sinks' dK and dV][the workspace of g4_attn_bwd] in the backward.
-static size_t sinks_bwd_front(const g4_problem& p) { return align256(g4::sinks_part_bytes(p)); }
+// [the sinks' dK and dV][their dS][the workspace of g4_attn_bwd] in the backward.
+static size_t sinks_bwd_front(const g4_problem& p) {
+  return align256(g4::sinks_part_bytes(p)) + align256(g4::sinks_ds_bytes(p));
+}
 
 size_t g4_sinks_workspace_bytes(const g4_problem* p, int32_t num_sinks, int phase) {
   g_last_error.clear();
@@ -1168,9 +1170,13 @@ int g4_attn_sinks_bwd(const g4_problem* p, int32_t num_sinks, const void* q, g4_
   const size_t front = sinks_bwd_front(*p);
   G4_TRY(check_sinks_ws(front + bwd_ws_bytes(*p), ws, ws_bytes));
   char* const base = (char*)ws + front;
-  // the window's part, with the whole rows' LSE and delta
-  G4_TRY(g4_attn_bwd(p, q, ql, k, kl, v, vl, o, ol, dout, dol, lse, dlse, dq, dql, dk, dkl, dv, dvl,
-                     base, ws_bytes - front, stream));
+  const size_t base_bytes = ws_bytes - front;
+  // dK and dV of the window with the whole rows' LSE and delta, then the sinks' over
+  // them, with their dS; dQ reads both
+  G4_TRY(g4_attn_bwd_delta(p, o, ol, dout, dol, dlse, base, base_bytes, stream));
+  G4_TRY(g4_attn_bwd_dkdv(p, q, ql, k, kl, v, vl, dout, dol, lse, dk, dkl, dv, dvl, base,
+                          base_bytes, stream));
+  G4_TRY(check_operand(dq, dql, "dq"));
   g4::BwdParams a{};
   fill_bwd(a, p, q, ql, k, kl, v, vl, base);
   a.dout = (const __bf16*)dout;
@@ -1182,8 +1188,12 @@ int g4_attn_sinks_bwd(const g4_problem* p, int32_t num_sinks, const void* q, g4_
   a.dv = (__bf16*)dv;
   a.dkl = dkl;
   a.dvl = dvl;
-  hipError_t e = g4::launch_sinks_bwd(a, num_sinks, (float*)ws, (hipStream_t)stream);
+  a.sinks = num_sinks;
+  if (a.ds != nullptr) a.sink_ds = (__bf16*)((char*)ws + align256(g4::sinks_part_bytes(*p)));
+  hipError_t e = g4::launch_sinks_bwd(a, (float*)ws, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "backward of the sinks");
+  e = g4::launch_bwd_dq(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "backward dQ with sinks");
   return G4_OK;
 }
 

@@ -1483,7 +1483,8 @@ struct DqRoles256Cfg {
   static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 };
 
-template <bool META>
+// SINKS: as FwdKernel's, the tile that holds the sinks comes before the window's.
+template <bool META, bool SINKS = false>
 struct DqRoles256Kernel {
   using C = DqRoles256Cfg;
   char G4_LDS* smem;
@@ -1501,6 +1502,13 @@ struct DqRoles256Kernel {
   TileCopier<C::kCPR, C::kBN, C::kNW> kcp, vcp;
   bf16x8 frag[C::kNC];  // Q (S waves) or dO (dP waves) fragments
   f32x16 acc[C::kNB];   // dQ^T over this wave's head-dim half
+  int sink_tiles;       // SINKS: 1 where the window begins behind them, else 0
+
+  // First key of tile `it` of the walk.
+  __device__ __forceinline__ int tile_key(int it, int t_first) const {
+    if constexpr (SINKS) return (it < sink_tiles ? it : t_first + it - sink_tiles) * C::kBN;
+    return (t_first + it) * C::kBN;
+  }
 
   __device__ __forceinline__ void issue_k(int row0, int buf) {
     kcp.issue_clamped(kbase + row0 * kstride, kstride, min(C::kBN, sq.lk - row0),
@@ -1518,7 +1526,8 @@ struct DqRoles256Kernel {
 
   // Rows of the tiles are keys 8 (r >> 2) + 4 h32 + (r & 3); lanes own queries.
   __device__ __forceinline__ void step(int cur, int it, int ntiles, int t_first) {
-    const int kb0 = (t_first + it) * C::kBN;
+    const int kb0 = tile_key(it, t_first);
+    const int kb1 = SINKS ? tile_key(it + 1, t_first) : kb0 + C::kBN;
     vm_wait<0>();
     barrier_lds();  // B1
     const char G4_LDS* kt = smem + C::kLdsK + cur * C::kTile;
@@ -1526,7 +1535,7 @@ struct DqRoles256Kernel {
 
     __builtin_amdgcn_sched_barrier(0);
     f32x16 part = f32x16{};
-    if (it + 1 < ntiles) issue_k(kb0 + C::kBN, cur ^ 1);
+    if (it + 1 < ntiles) issue_k(kb1, cur ^ 1);
     row_steps(rrd, role == 0 ? kt : vt, part, frag);
     __builtin_amdgcn_sched_barrier(0);
 
@@ -1551,7 +1560,8 @@ struct DqRoles256Kernel {
           float p = fast_exp2(part[r] * kLog2e - my_lse2);
           if (!full) {
             const int j = kb0 + jl0 + e;
-            const bool in_w = j >= lo_w;
+            bool in_w = j >= lo_w;
+            if constexpr (SINKS) in_w |= j < a->sinks;
             const bool causal = in_w & (j <= hi_c);
             const bool vis = has_vid & (my_vid >= 0) & (vk[e] == my_vid) & in_w & (j < sq.lk);
             const bool doc_ok = !has_doc | (dk[e] == my_doc);
@@ -1567,7 +1577,7 @@ struct DqRoles256Kernel {
       *(f32x4 G4_LDS*)xslot(own, q4) =
           f32x4{part[4 * q4], part[4 * q4 + 1], part[4 * q4 + 2], part[4 * q4 + 3]};
     barrier_lds();  // B2
-    if (it + 1 < ntiles) issue_v(kb0 + C::kBN);
+    if (it + 1 < ntiles) issue_v(kb1);
 
     // dS = P (dP - delta) from the same fp32 values in both waves of the group.
     bf16x8 dsb[2];
@@ -1589,9 +1599,9 @@ struct DqRoles256Kernel {
 };
 
 // Work item L: (KV head, sequence, query tile, head of the group).
-template <bool META, bool QUEUE>
+template <bool META, bool QUEUE, bool SINKS>
 __device__ __forceinline__ void dq_roles256_item(const BwdParams& a, char* smem_raw, int L) {
-  using K = DqRoles256Kernel<META>;
+  using K = DqRoles256Kernel<META, SINKS>;
   using C = DqRoles256Cfg;
   K ker;
   ker.smem = (char G4_LDS*)smem_raw;
@@ -1658,7 +1668,11 @@ __device__ __forceinline__ void dq_roles256_item(const BwdParams& a, char* smem_
   int klo, khi;
   query_tile_key_range(ker.a0, a_last_valid, sq.lk, p.window, span_max, klo, khi);
   const int t_first = klo / C::kBN;
-  const int ntiles = (khi + C::kBN - 1) / C::kBN - t_first;
+  int ntiles = (khi + C::kBN - 1) / C::kBN - t_first;
+  if constexpr (SINKS) {
+    ker.sink_tiles = min(t_first, 1);
+    ntiles += ker.sink_tiles;
+  }
   if (ker.has_doc &&
       doc_uniform<C::kNW>(p.document_ids, sq.ktok, sq.lk, min(klo / 64 * 64, ker.a0),
                           max((khi + 63) / 64 * 64, a_last_valid + 1), tid, ker.lane,
@@ -1697,8 +1711,8 @@ __device__ __forceinline__ void dq_roles256_item(const BwdParams& a, char* smem_
   for (int b = 0; b < C::kNB; ++b) ker.acc[b] = f32x16{};
 
   if (ntiles > 0) {
-    ker.issue_k(t_first * C::kBN, 0);
-    ker.issue_v(t_first * C::kBN);
+    ker.issue_k(ker.tile_key(0, t_first), 0);
+    ker.issue_v(ker.tile_key(0, t_first));
   }
   for (int it = 0; it < ntiles; ++it) ker.step(it & 1, it, ntiles, t_first);
 
@@ -1718,7 +1732,7 @@ __device__ __forceinline__ void dq_roles256_item(const BwdParams& a, char* smem_
 
 // Persistent: a few workgroups per CU take query-tile tickets from the dQ
 // work queue.
-template <bool META, bool QUEUE>
+template <bool META, bool QUEUE, bool SINKS = false>
 __global__ void __launch_bounds__(DqRoles256Cfg::kNT, 1) dq_roles256_kernel(BwdParams a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   // The recompute launch after a stored-dS pass takes its items from that
@@ -1732,11 +1746,11 @@ __global__ void __launch_bounds__(DqRoles256Cfg::kNT, 1) dq_roles256_kernel(BwdP
     for (;;) {
       const int t = wq.next((int G4_LDS*)smem_raw);
       if (t >= n) break;
-      dq_roles256_item<META, true>(a, smem_raw, t);
+      dq_roles256_item<META, true, SINKS>(a, smem_raw, t);
     }
   } else {
     const int t = xcd_remap(blockIdx.x, gridDim.x);
-    if (t < n) dq_roles256_item<META, false>(a, smem_raw, t);
+    if (t < n) dq_roles256_item<META, false, SINKS>(a, smem_raw, t);
   }
 }
 
@@ -1870,6 +1884,19 @@ struct DqDsKernel {
     }
   }
 
+  // The sinks behind the window (BwdParams::sink_ds): keys 0 .. 63 of the sequence, of
+  // which the first 32 have dS, and the 2 KB tiles of the rows that reach past them.
+  __device__ __forceinline__ void issue_sinks(const char* ds_row, bool copied, int buf) {
+    kcp.issue_clamped(kbase, kstride, min(C::kBN, sq.lk), smem + C::kLdsK + buf * C::kKTile);
+    if (!copied) return;
+    const int g = wave >> 1, half = (wave & 1) * 1024;
+#pragma unroll
+    for (int h = 0; h < C::kHeads; ++h)
+      if (h < nh)
+        b2l16_nt(ds_row + h * (int64_t)a->ds_rows * 2048, (uint32_t)(half + lane * 16),
+                 smem + C::kLdsDs + ((buf * C::kHeads + h) * 4 + g) * 4096 + half);
+  }
+
   template <int KS>
   __device__ __forceinline__ void kstep(const char G4_LDS* kt_tile, const char G4_LDS* dsb,
                                         bool v0, bool v1) {
@@ -1957,7 +1984,8 @@ __host__ __device__ __forceinline__ int dq_ds_heads(const g4_problem& p) {
 // are read once into that XCD's L2 (config 3 dQ 0.257 -> 0.227 ms; the same
 // order at head dim 512 measured 0.98 -> 1.03 ms on config 2: there the
 // heaviest-first order across heads matters more).
-template <int D, bool QUEUE>
+// SINKS (head dim 256, no key metadata): the sinks' tile comes before the band's.
+template <int D, bool QUEUE, bool SINKS>
 __device__ __forceinline__ void dq_ds_item(const BwdParams& a, char* smem_raw, int L,
                                            const SeqTiles& tiles, bool compact) {
   using C = DqDsCfg<D>;
@@ -2065,7 +2093,27 @@ __device__ __forceinline__ void dq_ds_item(const BwdParams& a, char* smem_raw, i
       for (int b = 0; b < C::kNBw; ++b) ker.acc[h][g][b] = f32x16{};
 
   const int g0 = 2 * ker.qpair;
-  if (kt_begin < nkt) ker.issue(kt_begin, 0);
+  if constexpr (SINKS) {
+    // row g has sinks behind its window when its last query has
+    auto far = [&](int g) {
+      return i0 + 32 * g < sq.lq && min(i0 + 32 * g + 32, sq.lq) - 1 + off >= p.window;
+    };
+    const bool any = min(i0 + C::kBM, sq.lq) - 1 + off >= p.window;
+    if (any)
+      ker.issue_sinks((const char*)a.sink_ds + ((int64_t)qh * a.ds_rows + row0 + gc) * 2048,
+                      far(gc), 1);
+    if (kt_begin < nkt) ker.issue(kt_begin, 0);
+    if (any) {
+      vm_wait<0>();
+      barrier_lds();
+      const char G4_LDS* ktile = ker.smem + C::kLdsK + C::kKTile;
+      const char G4_LDS* ds0 = ker.smem + C::kLdsDs + (C::kHeads * 4 + g0) * 4096;
+      ker.template kstep<0>(ktile, ds0, far(g0), far(g0 + 1));
+      ker.template kstep<1>(ktile, ds0, far(g0), far(g0 + 1));
+    }
+  } else {
+    if (kt_begin < nkt) ker.issue(kt_begin, 0);
+  }
   for (int kt = kt_begin; kt < nkt; ++kt) {
     const int cur = (kt - kt_begin) & 1;
     vm_wait<0>();
@@ -2136,7 +2184,7 @@ __device__ __forceinline__ void dq_ds_item(const BwdParams& a, char* smem_raw, i
 // Persistent (QUEUE): a few workgroups per CU take items from the dQ work
 // queue: head dim 512 the heaviest tiles first from one queue, head dim 256
 // each XCD from its own contiguous run (XcdQueue).
-template <int D, bool QUEUE>
+template <int D, bool QUEUE, bool SINKS = false>
 __global__ void __launch_bounds__(DqDsCfg<D>::kNT, 1) dq_ds_kernel(BwdParams a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   if constexpr (QUEUE) {
@@ -2151,25 +2199,25 @@ __global__ void __launch_bounds__(DqDsCfg<D>::kNT, 1) dq_ds_kernel(BwdParams a) 
       PrefetchQueue q{a.sched + 2, n};
       for (int t = q.first(); q.valid(t); t = q.next((int G4_LDS*)smem_raw)) {
         q.draw();
-        dq_ds_item<D, true>(a, smem_raw, t, tiles, false);
+        dq_ds_item<D, true, SINKS>(a, smem_raw, t, tiles, false);
       }
     } else {
       XcdQueue q{a.sched + kDqXcdQueue, n};
       q.draw();
       for (int t = q.next((int G4_LDS*)smem_raw); t >= 0; t = q.next((int G4_LDS*)smem_raw)) {
         q.draw();
-        dq_ds_item<D, true>(a, smem_raw, t, tiles, compact);
+        dq_ds_item<D, true, SINKS>(a, smem_raw, t, tiles, compact);
       }
     }
   } else {
-    dq_ds_item<D, false>(a, smem_raw, xcd_remap(blockIdx.x, gridDim.x), SeqTiles{}, false);
+    dq_ds_item<D, false, SINKS>(a, smem_raw, xcd_remap(blockIdx.x, gridDim.x), SeqTiles{}, false);
   }
 }
 
 }  // namespace
 
 
-template <int D>
+template <int D, bool SINKS = false>
 static hipError_t launch_dq_ds(const BwdParams& a, hipStream_t stream) {
   using C = DqDsCfg<D>;
   static LdsAttr attr[2];
@@ -2182,9 +2230,9 @@ static hipError_t launch_dq_ds(const BwdParams& a, hipStream_t stream) {
   static PersistentGrid grid;
   bool queue = false;
   const int64_t nblocks =
-      grid.size((const void*)dq_ds_kernel<D, true>, C::kNT, C::kLdsBytes, items, &queue);
+      grid.size((const void*)dq_ds_kernel<D, true, SINKS>, C::kNT, C::kLdsBytes, items, &queue);
   if (nblocks <= 0) return hipErrorInvalidValue;
-  void (*kern)(BwdParams) = queue ? dq_ds_kernel<D, true> : dq_ds_kernel<D, false>;
+  void (*kern)(BwdParams) = queue ? dq_ds_kernel<D, true, SINKS> : dq_ds_kernel<D, false, SINKS>;
   hipError_t e = attr[queue].ensure((const void*)kern, C::kLdsBytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(C::kNT), C::kLdsBytes, stream, b);
@@ -2205,6 +2253,12 @@ hipError_t launch_dq_roles_d(const BwdParams& a, hipStream_t stream) {
   void (*kern)(BwdParams);
   if constexpr (D == 512) {
     kern = meta ? dq_roles_kernel<true> : dq_roles_kernel<false>;
+  } else if (a.sinks > 0) {
+    static PersistentGrid grid;
+    nblocks = grid.size((const void*)dq_roles256_kernel<false, true, true>, C::kNT, C::kLdsBytes,
+                        items, &queue);
+    if (nblocks <= 0) return hipErrorInvalidValue;
+    kern = queue ? dq_roles256_kernel<false, true, true> : dq_roles256_kernel<false, false, true>;
   } else {
     static PersistentGrid grid;
     nblocks = grid.size((const void*)(meta ? dq_roles256_kernel<true, true>
@@ -2214,8 +2268,9 @@ hipError_t launch_dq_roles_d(const BwdParams& a, hipStream_t stream) {
     kern = meta ? (queue ? dq_roles256_kernel<true, true> : dq_roles256_kernel<true, false>)
                 : (queue ? dq_roles256_kernel<false, true> : dq_roles256_kernel<false, false>);
   }
-  static LdsAttr attr[4];
-  hipError_t e = attr[2 * meta + queue].ensure((const void*)kern, C::kLdsBytes);
+  static LdsAttr attr[6];
+  hipError_t e =
+      attr[(a.sinks > 0 ? 4 : 2 * meta) + queue].ensure((const void*)kern, C::kLdsBytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(C::kNT), C::kLdsBytes, stream, b);
   return hipGetLastError();
@@ -2236,6 +2291,7 @@ hipError_t launch_bwd_dq(const BwdParams& a, hipStream_t stream) {
   }
   if (a.p.head_dim == 256) {
     if (a.ds == nullptr) return launch_dq_roles_d<256>(a, stream);
+    if (a.sinks > 0) return launch_dq_ds<256, true>(a, stream);
     if (a.dq_list != nullptr && !a.dq_list_clear) {
       // The list is refilled by every stored-dS pass (a fill kernel, not a
       // memset node, so the launch sequence can be captured in a graph).

@@ -126,6 +126,13 @@ struct BwdParams {
   // The delta pass of this very call has just cleared the list's counter (the
   // dQ stage on its own clears it first).
   bool dq_list_clear;
+  // Head dim 256 with a window, without key metadata: the first `sinks` keys of a
+  // sequence stay visible (0: the plain window).  With stored dS, sink_ds holds the
+  // sinks' tiles for the dQ stage: [32 keys][32 positions] bf16 in the band's order, of
+  // row r and query head h at (h * ds_rows + r) * 2 KB, pairs inside the window as
+  // zeros; only rows with a sink behind their window are written and read.
+  int sinks;
+  __bf16* sink_ds;
 };
 
 // Workspace layout helpers (bytes).
@@ -249,11 +256,12 @@ hipError_t launch_bwd_dq(const BwdParams& a, hipStream_t stream);
 // The sinks' part of the backward at head dim 256 with a window (g4_sinks.hip).
 struct SinkParams {
   BwdParams b;
-  int sinks, chunk;  // keys; queries of a workgroup
-  float* part;       // the chunks' dK and dV
+  int chunk;    // queries of a workgroup
+  float* part;  // the chunks' dK and dV
 };
 size_t sinks_part_bytes(const g4_problem& p);
-hipError_t launch_sinks_bwd(const BwdParams& b, int sinks, float* part, hipStream_t stream);
+size_t sinks_ds_bytes(const g4_problem& p);  // 0: no stored dS
+hipError_t launch_sinks_bwd(const BwdParams& b, float* part, hipStream_t stream);
 hipError_t launch_mask(const g4_problem& p, uint8_t* out, const int* span_lo, const int* span_hi,
                        hipStream_t stream);
 hipError_t launch_ranges(const g4_problem& p, int direction, int row_tile, int32_t* out,

@@ -5,16 +5,16 @@
 // and delta of the whole row, P = exp(S - LSE) and dS = P (dP - delta) of a pair
 // do not depend on which other pairs the row has.  What is left, for sequences
 // longer than the window:
-//   dQ += dS K over the sinks behind the window (added to the stored rows), and
 //   dK, dV of the sinks, over every query of the sequence (written anew, so that
-//   each is one fp32 sum rounded once).
+//   each is one fp32 sum rounded once), and
+//   their dS behind the window, stored as bf16 tiles that the dQ stage adds to the
+//   window's as one more key tile (without stored dS that stage recomputes them).
 // A workgroup takes a chunk of a sequence's queries and one KV head; its waves
 // take 32 rows of one query head at a time: S = Q K^T and dP = dO V^T with keys
-// along lanes feed dV^T += dO^T P and dK^T += Q^T dS from registers, the same
-// products with the operands exchanged (S^T, dP^T: queries along lanes) feed
-// dQ^T = K^T dS^T.  The chunk's dK and dV go to the workspace and a second launch
-// adds the chunks in order (no atomics).  Bound by HBM: Q, dO and dQ are read and
-// dQ is written once more, 4 x 512 bytes a row.
+// along lanes feed dV^T += dO^T P and dK^T += Q^T dS from registers.  The chunk's
+// dK and dV go to the workspace and a second launch adds the chunks in order (no
+// atomics).  Bound by HBM: Q and dO are read once more, 2 x 512 bytes a row, and
+// 64 bytes of dS written.
 #include "g4_kernels.h"
 
 namespace g4 {
@@ -28,8 +28,7 @@ constexpr int kNB = D / 32;  // 32-wide blocks of the head dim
 constexpr int kWaves = 4;
 constexpr int kRowsBytes = 32 * D * 2;            // a tile of Q or dO
 constexpr int kWaveBytes = 2 * kRowsBytes;        // = 32 fp32 rows of D
-constexpr int kLdsK = kWaves * kWaveBytes;
-constexpr int kLdsStat = kLdsK + kRowsBytes;      // [wave][LSE x 32 | delta x 32] fp32
+constexpr int kLdsStat = kWaves * kWaveBytes;     // [wave][LSE x 32 | delta x 32] fp32
 constexpr int kLdsBytes = kLdsStat + kWaves * 256;
 static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 static_assert(kWaveBytes == 32 * D * 4, "the sums of a wave fit its tiles");
@@ -76,45 +75,18 @@ __device__ __forceinline__ int sink_slots_before(const SinkParams& a, int s) {
   return __builtin_amdgcn_readfirstlane(n);
 }
 
-// x = rows . keys^T (keys along lanes) and, with BOTH, y = keys . rows^T; the keys'
-// fragments from `keys`, a tile in LDS (K) or registers (V).
+// x += rows . keys^T over the steps CP .. kNC - 1.
 template <int CP, class RR>
-__device__ __forceinline__ bf16x8 sink_fragment(const RR& rrd, const char G4_LDS* t) {
-  return rrd.template read<0, 0, CP>(t);
-}
-template <int CP, class RR>
-__device__ __forceinline__ bf16x8 sink_fragment(const RR&, const bf16x8 (&f)[kNC]) {
-  return f[CP];
-}
-template <bool BOTH, int CP, class RR, class Keys>
-__device__ __forceinline__ void sink_products(const RR& rrd, const char G4_LDS* rows,
-                                              const Keys& keys, f32x16& x, f32x16& y) {
+__device__ __forceinline__ void sink_product(const RR& rrd, const char G4_LDS* rows,
+                                             const bf16x8 (&keys)[kNC], f32x16& x) {
   if constexpr (CP < kNC) {
-    const bf16x8 f = rrd.template read<0, 0, CP>(rows), g = sink_fragment<CP>(rrd, keys);
-    x = mfma32(f, g, x);
-    if constexpr (BOTH) y = mfma32(g, f, y);
-    sink_products<BOTH, CP + 1>(rrd, rows, keys, x, y);
+    x = mfma32(rrd.template read<0, 0, CP>(rows), keys[CP], x);
+    sink_product<CP + 1>(rrd, rows, keys, x);
   }
 }
 
 // Byte of the 16-byte chunk c of fp32 row r in a wave's area (D * 4 bytes a row).
 __device__ __forceinline__ int sum_off(int r, int c) { return r * D * 4 + (c ^ r) * 16; }
-
-template <int B, class TR>
-__device__ __forceinline__ void sink_dq(const TR& trd, const char G4_LDS* kt,
-                                        const bf16x8 (&ds)[2], char G4_LDS* stage, int l32,
-                                        int h32) {
-  if constexpr (B < kNB) {
-    f32x16 acc = {};
-    acc = mfma32(trd.template read<0, 0, B>(kt), ds[0], acc);
-    acc = mfma32(trd.template read<16, 0, B>(kt), ds[1], acc);
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4)
-      *(f32x4 G4_LDS*)(stage + sum_off(l32, 8 * B + 2 * r4 + h32)) =
-          f32x4{acc[4 * r4], acc[4 * r4 + 1], acc[4 * r4 + 2], acc[4 * r4 + 3]};
-    sink_dq<B + 1>(trd, kt, ds, stage, l32, h32);
-  }
-}
 
 }  // namespace
 
@@ -131,38 +103,30 @@ __global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
   const Seq sq = resolve_seq(p, s);
   const int off = sq.lk - sq.lq;
   const int grp = p.num_q_heads / p.num_kv_heads;
-  const int sinks = min(sp.sinks, sq.lk);
+  const int sinks = min(a.sinks, sq.lk);
 
-  // ---- the sinks' K and V: rows past them as zeros -----------------------------
-  const __bf16* kbase = a.k + tok_off(sq, s, sq.ktok, 0, a.kl) + (int64_t)kvh * a.kl.head_stride;
-  const __bf16* vbase = a.v + tok_off(sq, s, sq.ktok, 0, a.vl) + (int64_t)kvh * a.vl.head_stride;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = i * 256 + tid, r = x / 32, c = x % 32;
-    const bf16x8 y = r < sinks ? ld_global16(kbase + r * a.kl.token_stride + c * 8) : bf16x8{};
-    *(bf16x8 G4_LDS*)(smem + kLdsK + (r * 32 + swz_slot(r, c)) * 16) = y;
-  }
-  bf16x8 vf[kNC];
+  // ---- the sinks' K and V along lanes (rows past them are masked) ---------------
+  bf16x8 kf[kNC], vf[kNC];
   {
-    const __bf16* vrow = vbase + min(l32, sinks - 1) * a.vl.token_stride + h32 * 8;
+    const int r = min(l32, sinks - 1);
+    const __bf16* krow = a.k + tok_off(sq, s, sq.ktok, r, a.kl) + (int64_t)kvh * a.kl.head_stride;
+    const __bf16* vrow = a.v + tok_off(sq, s, sq.ktok, r, a.vl) + (int64_t)kvh * a.vl.head_stride;
 #pragma unroll
     for (int c = 0; c < kNC; ++c) {
-      const bf16x8 y = ld_global16(vrow + c * 16);
-      vf[c] = l32 < sinks ? y : bf16x8{};
+      kf[c] = ld_global16(krow + 16 * c + 8 * h32);
+      vf[c] = ld_global16(vrow + 16 * c + 8 * h32);
     }
   }
-  barrier_lds();
   RowReader<32> rrd;
   TrReader<32> trd;
   rrd.init(lane);
   trd.init(lane);
-  const char G4_LDS* const kt = smem + kLdsK;
 
   // ---- the chunk's rows -----------------------------------------------------------
   char G4_LDS* const qt = smem + wave * kWaveBytes;
   char G4_LDS* const dot = qt + kRowsBytes;
   float G4_LDS* const stat = (float G4_LDS*)(smem + kLdsStat + wave * 256);
-  TileCopier<32, 32, 1> qcp, docp;
+  TileCopier<32, 32, 1, true> qcp, docp;
   qcp.init(a.ql.token_stride, 0, lane);
   docp.init(a.dol.token_stride, 0, lane);
   f32x16 dk[kNB], dv[kNB];
@@ -196,16 +160,10 @@ __global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
     wait_lds();
 
     const int a0 = i0 + off;
-    const bool far = a0 + nrows - 1 >= p.window;  // a row with sinks behind its window
-    f32x16 sc = {}, st = {}, dp = {}, dpt = {};
-    if (far) {
-      sink_products<true, 0>(rrd, qt, kt, sc, st);
-      sink_products<true, 0>(rrd, dot, vf, dp, dpt);
-    } else {
-      sink_products<false, 0>(rrd, qt, kt, sc, st);
-      sink_products<false, 0>(rrd, dot, vf, dp, dpt);
-    }
-    bf16x8 pb[2], dsb[2], dst[2];
+    f32x16 sc = {}, dp = {};
+    sink_product<0>(rrd, qt, kf, sc);
+    sink_product<0>(rrd, dot, vf, dp);
+    bf16x8 pb[2], dsb[2], behind[2];  // P, dS, dS behind the window
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const f32x4 lse = *(const f32x4 G4_LDS*)(stat + 8 * r4 + 4 * h32);
@@ -218,54 +176,20 @@ __global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
         const float ds = ok ? pr * (dp[r] - dl[e]) : 0.f;
         pb[r / 8][r % 8] = (__bf16)pr;
         dsb[r / 8][r % 8] = (__bf16)ds;
+        behind[r / 8][r % 8] = (__bf16)(l32 <= a0 + row - p.window ? ds : 0.f);
       }
     }
-    if (far) {
-      const float lse = stat[l32], dl = stat[32 + l32];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = 8 * (r / 4) + 4 * h32 + r % 4;
-        const bool ok = (key < sinks) & (key <= a0 + l32 - p.window);
-        const float pr = ok ? fast_exp2(__builtin_fmaf(st[r], kLog2e, -lse)) : 0.f;
-        dst[r / 8][r % 8] = (__bf16)(ok ? pr * (dpt[r] - dl) : 0.f);
-      }
+    if (a.sink_ds != nullptr && a0 + nrows - 1 >= p.window) {
+      // (queries in accumulator order: a lane's 16 are one run)
+      const int64_t row = (sq.packed ? sq.qtok / 32 + s : (int64_t)s * ((p.seqlen_q + 31) / 32)) +
+                          i0 / 32;
+      bf16x8* const out =
+          (bf16x8*)(a.sink_ds + ((int64_t)qh * a.ds_rows + row) * 1024 + l32 * 32 + h32 * 16);
+      out[0] = behind[0];
+      out[1] = behind[1];
     }
     acc_steps<kNB>(trd, dot, pb, dv);
     acc_steps<kNB>(trd, qt, dsb, dk);
-    if (far) {
-      // dQ's rows in fp32 over the tiles just used, then whole rows added to memory.
-      // (The lane passes through an empty asm: the swizzled offsets derived from it are
-      // formed here, not held in registers across the loop.)
-      wait_lds();
-      int ln = lane;
-      asm volatile("" : "+v"(ln));
-      const int l32 = ln & 31, h32 = ln >> 5;
-      sink_dq<0>(trd, kt, dst, qt, l32, h32);
-      __bf16* const dqrow = a.dq + tok_off(sq, s, sq.qtok, i0, a.dql) +
-                            (int64_t)qh * a.dql.head_stride + l32 * 8;
-      wait_lds();
-#pragma unroll 1
-      for (int j = 0; j < 16; j += 8) {
-        bf16x8 y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          y[i] = ld_global16(dqrow +
-                             (int64_t)min(2 * (j + i) + h32, nrows - 1) * a.dql.token_stride);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = 2 * (j + i) + h32;
-          const f32x4 u = *(const f32x4 G4_LDS*)(qt + sum_off(row, 2 * l32));
-          const f32x4 v = *(const f32x4 G4_LDS*)(qt + sum_off(row, 2 * l32 + 1));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[i][e] = (__bf16)((float)y[i][e] + u[e]);
-            y[i][4 + e] = (__bf16)((float)y[i][4 + e] + v[e]);
-          }
-          // (a row before the window's reach gets zeros added: its bits stay)
-          if (row < nrows) *(bf16x8*)(dqrow + (int64_t)row * a.dql.token_stride) = y[i];
-        }
-      }
-    }
   }
 
   // ---- the waves' sums, key by key --------------------------------------------------
@@ -298,7 +222,7 @@ __global__ void __launch_bounds__(64) sinks_sum_kernel(SinkParams sp) {
   const BwdParams& a = sp.b;
   const g4_problem& p = a.p;
   const int kvh = blockIdx.x % p.num_kv_heads, s = blockIdx.x / p.num_kv_heads;
-  const int r = blockIdx.y % sp.sinks, which = blockIdx.y / sp.sinks;
+  const int r = blockIdx.y % a.sinks, which = blockIdx.y / a.sinks;
   const int n = sink_chunks(sp, s);
   const Seq sq = resolve_seq(p, s);
   if (n == 0 || r >= sq.lk) return;
@@ -331,8 +255,16 @@ size_t sinks_part_bytes(const g4_problem& p) {
   return (size_t)sink_slots(p) * p.num_kv_heads * 2 * kSinkKeys * D * 4;
 }
 
-hipError_t launch_sinks_bwd(const BwdParams& b, int sinks, float* part, hipStream_t stream) {
-  SinkParams a{b, sinks, sink_chunk(b.p), part};
+// A 2 KB tile per (32-query row, query head), where dS is stored.
+size_t sinks_ds_bytes(const g4_problem& p) {
+  if (!ds_bytes(p)) return 0;
+  int rows, cols;
+  ds_geometry(p, &rows, &cols);
+  return (size_t)rows * p.num_q_heads * 2048;
+}
+
+hipError_t launch_sinks_bwd(const BwdParams& b, float* part, hipStream_t stream) {
+  SinkParams a{b, sink_chunk(b.p), part};
   const int64_t blocks = sink_slots(b.p) * b.p.num_kv_heads;
   if (blocks <= 0) return hipSuccess;  // no sequence is longer than the window
   static LdsAttr attr;
@@ -342,7 +274,7 @@ hipError_t launch_sinks_bwd(const BwdParams& b, int sinks, float* part, hipStrea
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(sinks_sum_kernel, dim3((unsigned)(b.p.num_seqs * b.p.num_kv_heads),
-                                            (unsigned)(2 * sinks)),
+                                            (unsigned)(2 * b.sinks)),
                      dim3(64), 0, stream, a);
   return hipGetLastError();
 }
