@@ -977,10 +977,73 @@ static g4::CacheAttnParams cache_attn_params(const g4_cache_attn& p) {
   return a;
 }
 
+// Larger chunks of new tokens: the visible rows of every sequence as bf16 in the
+// workspace, and the forward of g4_attn_fwd over them.  Reading pages as they lie
+// costs the whole cache once per group of 16 query rows, the copy five times its
+// bytes once.
+struct CacheExpand {
+  static constexpr int kRows = 64;  // query rows of a KV head from which on it is taken
+  static constexpr size_t kMost = size_t(8) << 30;  // bytes of rows at most
+  g4_problem p;
+  int64_t rows;       // of K and of V in the workspace
+  size_t cu, operand, fwd;  // bytes of the lengths, of K or V, of the forward's workspace
+  bool used;
+  explicit CacheExpand(const g4_cache_attn& a) {
+    const int hkv = a.cache.num_kv_heads, d = a.cache.head_dim;
+    const int64_t see = a.window > 0 ? (int64_t)a.window + a.max_seqlen_q + a.num_sinks
+                                     : (int64_t)a.max_seqlen_k;
+    const int64_t most = std::min<int64_t>(a.max_seqlen_k, see);
+    rows = most * a.table.batch;
+    operand = align256((size_t)rows * hkv * d * 2);
+    cu = align256((size_t)(a.table.batch + 1) * 4);
+    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > kRows && 2 * operand <= kMost &&
+           rows < 0x7fffffffLL && (int64_t)hkv * d < (int64_t(1) << 24) &&
+           (int64_t)a.table.batch * a.max_seqlen_q < 0x7fffffffLL;
+    p = g4_problem{};
+    p.num_seqs = a.table.batch;
+    p.seqlen_q = a.max_seqlen_q;
+    p.seqlen_k = (int32_t)most;
+    p.num_q_heads = a.num_q_heads;
+    p.num_kv_heads = hkv;
+    p.head_dim = d;
+    p.window = a.window;
+    p.total_q = a.total_q;
+    p.total_k = rows;
+    p.lse_head_stride = a.total_q;
+    fwd = 0;
+    if (used)
+      fwd = a.num_sinks > 0 ? align256(g4::split_bytes(p, 1)) : align256(fwd_split_ws_bytes(p));
+  }
+  size_t bytes() const { return 2 * cu + 2 * operand + fwd; }
+};
+
 size_t g4_cache_attn_workspace_bytes(const g4_cache_attn* p) {
   g_last_error.clear();
   if (check_cache_attn(p) != G4_OK) return 0;
-  return align256(g4::cache_part_bytes(cache_attn_params(*p)));
+  const CacheExpand x(*p);
+  return x.used ? x.bytes() : align256(g4::cache_part_bytes(cache_attn_params(*p)));
+}
+
+static int cache_attn_expanded(const g4_cache_attn& p, CacheExpand& x, const void* q, g4_layout ql,
+                               void* o, g4_layout ol, float* lse, char* ws, hipStream_t st) {
+  int* const cu_q = (int*)ws;
+  int* const cu_k = (int*)(ws + x.cu);
+  __bf16* const k = (__bf16*)(ws + 2 * x.cu);
+  __bf16* const v = (__bf16*)(ws + 2 * x.cu + x.operand);
+  char* const fwd = ws + 2 * x.cu + 2 * x.operand;
+  const int hkv = p.cache.num_kv_heads, d = p.cache.head_dim;
+  const g4_layout lay{0, (int64_t)hkv * d, d};
+  g4::ExpandParams e{p.table, p.cu_seqlens_q, p.total_q, p.max_seqlen_q, p.max_seqlen_k,
+                     p.window, p.num_sinks, x.p.seqlen_k, cu_q, cu_k};
+  hipError_t err = g4::launch_cache_expand_lengths(e, st);
+  if (err != hipSuccess) return hip_fail(err, "cache attention lengths");
+  g4::GatherParams g{p.cache, p.table, cu_k, x.rows, {k, v}, {lay, lay}, cu_q, p.max_seqlen_k,
+                     p.window, p.num_sinks};
+  err = g4::launch_cache_gather(g, st);
+  if (err != hipSuccess) return hip_fail(err, "cache attention rows");
+  x.p.cu_seqlens_q = cu_q;
+  x.p.cu_seqlens_k = cu_k;
+  return fwd_impl(&x.p, q, ql, k, lay, v, lay, o, ol, lse, fwd, x.fwd, st, p.num_sinks);
 }
 
 int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void* o, g4_layout ol,
@@ -992,12 +1055,15 @@ int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void*
   G4_TRY(check_operand(o, ol, "o"));
   if (lse == nullptr) return fail(G4_ERR_INVALID, "lse is NULL");
   g4::CacheAttnParams a = cache_attn_params(*p);
-  const size_t need = align256(g4::cache_part_bytes(a));
+  CacheExpand x(*p);
+  const size_t need = x.used ? x.bytes() : align256(g4::cache_part_bytes(a));
   if (ws == nullptr || ws_bytes < need || ((uintptr_t)ws) % 256) {
     char buf[128];
     snprintf(buf, sizeof buf, "%zu bytes at 256 needed, %zu given", need, ws_bytes);
     return fail(G4_ERR_WORKSPACE, "cache attention workspace: %s", buf);
   }
+  if (x.used)
+    return cache_attn_expanded(*p, x, q, ql, o, ol, lse, (char*)ws, (hipStream_t)stream);
   a.q = (const __bf16*)q;
   a.o = (__bf16*)o;
   a.lse = lse;

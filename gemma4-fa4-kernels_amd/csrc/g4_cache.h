@@ -87,8 +87,36 @@ struct GatherParams {
   int64_t total;
   __bf16* out[2];
   g4_layout lay[2];
+  // For attention of the queries cu_q (null: every token): of each sequence only what
+  // they can see (VisibleRows), and K of a token without a page as NaN.
+  const int* cu_q;
+  int max_k, window, sinks;
 };
 hipError_t launch_cache_gather(const GatherParams& a, hipStream_t stream);
+
+// The tokens that nq last queries of a sequence of len tokens can see, closed up:
+// rows 0 .. sinks - 1 are the sinks, then row x is token x + shift.  Distances
+// between queries and the window's keys stay what they were.
+struct VisibleRows {
+  int shift, n;
+  __device__ __forceinline__ void init(int len, int nq, int window, int sinks) {
+    const int lo = window > 0 ? max(len - nq - window + 1, 0) : 0;
+    shift = max(lo - sinks, 0);
+    n = len - shift;
+  }
+};
+
+// Cumulative lengths of the closed-up sequences and of the queries, both within
+// their buffers whatever the lengths on the device are.
+struct ExpandParams {
+  g4_page_table tab;
+  const int* cu_q;
+  int64_t total_q;
+  int max_q, max_k, window, sinks;
+  int most_k;  // rows of a sequence at most
+  int *out_q, *out_k;  // (batch + 1) each
+};
+hipError_t launch_cache_expand_lengths(const ExpandParams& a, hipStream_t stream);
 
 // Attention of new tokens over the cached ones.
 struct CacheAttnParams {

@@ -127,18 +127,26 @@ __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {
   const int row0 = a.cu[s], n = a.cu[s + 1] - row0;
   const int rel = slot - (row0 / 32 + s);
   if (rel < 0 || rel >= (n + 31) / 32) return;
-  const int len = a.tab.seq_lens[s];
+  int len = a.tab.seq_lens[s], shift = 0;
+  if (a.cu_q != nullptr) {
+    VisibleRows v;
+    len = min(max(len, 0), a.max_k);
+    v.init(len, a.cu_q[s + 1] - a.cu_q[s], a.window, a.sinks);
+    shift = v.shift;
+  }
   const int tid = threadIdx.x, sub = tid / kLanes, col = tid % kLanes;
   const uint8_t* in = (const uint8_t*)(which ? c.v : c.k) + col * 8;
   const float* scales = which ? c.v_scale : c.k_scale;
   __bf16* out = a.out[which] + (int64_t)head * a.lay[which].head_stride + col * 8;
 #pragma unroll
   for (int i = 0; i < kCacheBlock / kRows; ++i) {
-    const int t = rel * 32 + i * kRows + sub;
-    const int64_t row = (int64_t)row0 + t;
-    if (t >= n || row < 0 || row >= a.total) continue;
+    const int x = rel * 32 + i * kRows + sub;
+    const int64_t row = (int64_t)row0 + x;
+    if (x >= n || row < 0 || row >= a.total) continue;
+    const int t = a.cu_q != nullptr && x >= a.sinks ? x + shift : x;
     const int page = t < len ? page_of(a.tab, c, s, t) : -1;
-    u32x4 y = {};
+    const uint32_t none = a.cu_q != nullptr && which == 0 ? 0x7fc07fc0u : 0u;  // NaN or 0
+    u32x4 y = {none, none, none, none};
     if (page >= 0) {
       const int64_t ph = (int64_t)page * c.num_kv_heads + head;
       const int at = t % c.page_size;
@@ -149,6 +157,49 @@ __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {
     }
     *(u32x4*)(out + row * a.lay[which].token_stride) = y;
   }
+}
+
+// One workgroup: prefix sums over the sequences.
+__global__ void __launch_bounds__(256) expand_lengths_kernel(ExpandParams a) {
+  __shared__ int64_t lds[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t base_q = 0, base_k = 0;
+  for (int s0 = 0; s0 < a.tab.batch; s0 += 256) {
+    const int s = s0 + tid;
+    int64_t q = 0, k = 0;
+    if (s < a.tab.batch) {
+      const int nq = (int)min(max((int64_t)a.cu_q[s + 1] - a.cu_q[s], (int64_t)0), (int64_t)a.max_q);
+      VisibleRows v;
+      v.init(min(max(a.tab.seq_lens[s], 0), a.max_k), nq, a.window, a.sinks);
+      q = nq;
+      k = min(v.n, a.most_k);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(q, o, 64), y = __shfl_up(k, o, 64);
+      if (lane >= o) q += x, k += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[0][wave] = q, lds[1][wave] = k;
+    __syncthreads();
+    int64_t before_q = base_q, before_k = base_k;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before_q += lds[0][w], before_k += lds[1][w];
+      base_q += lds[0][w];
+      base_k += lds[1][w];
+    }
+    if (s < a.tab.batch) {
+      a.out_q[s + 1] = (int)min(before_q + q, a.total_q);
+      a.out_k[s + 1] = (int)(before_k + k);
+    }
+  }
+  if (tid == 0) a.out_q[0] = a.out_k[0] = 0;
+}
+
+hipError_t launch_cache_expand_lengths(const ExpandParams& a, hipStream_t stream) {
+  hipLaunchKernelGGL(expand_lengths_kernel, dim3(1), dim3(256), 0, stream, a);
+  return hipGetLastError();
 }
 
 hipError_t launch_cache_gather(const GatherParams& a, hipStream_t stream) {

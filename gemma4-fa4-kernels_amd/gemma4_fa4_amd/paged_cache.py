@@ -214,11 +214,15 @@ def paged_cache_attention(
     A query at position ``a`` sees token ``j <= a``; with ``sliding_window`` W only
     ``j > a - W`` or ``j < num_sinks`` (up to 32), and pages that no query sees any more
     may be gone (``release_pages``).  Returns bf16 O like ``q`` and fp32 LSE ``(Hq, T)``:
-    0 and -inf for a query that sees nothing, NaN where a visible token has no page;
+    0 and -inf for a query that sees nothing, NaN in O where a visible token has no page;
     rows past ``cu_seqlens_q[-1]`` are not written.  ``max_seqlen_q`` and
     ``max_seqlen_k`` are bounds of the lengths on the device, which no call reads on the
     host; a batch beyond them gets unspecified rows.  Head dim 512 takes neither
     window nor sinks; query heads are 1, 2, 4 or 8 times the cache's.
+
+    A few new tokens per sequence are computed from the pages as they lie; from more
+    than 64 query rows per KV head on, what the batch can see is laid out as bf16 rows
+    in a workspace (``4 * batch * tokens * Hkv * head_dim`` bytes, up to 8 GiB).
     """
     if q.ndim != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be a rank-3 BF16 (T, H, D) tensor")

@@ -385,10 +385,10 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table,
  * sits at position a = seq_lens[b] - (queries of b) + i, and sees token j <= a
  * with j > a - window (window > 0) or j < num_sinks.  O bf16, LSE fp32 (heads,
  * total_q); a query that sees no token gets 0 and -inf, one that sees a token
- * without a page NaN.  Sequences of one to a few queries are read from the pages
+ * without a page NaN in O.  Sequences of one to a few queries are read from the pages
  * as they lie; larger chunks as bf16 rows in the workspace, through the forward
  * of g4_attn_fwd.  max_seqlen_q / max_seqlen_k bound the batch's (device)
- * lengths: queries and tokens past them are not read, written or seen.
+ * lengths (a batch beyond them gets unspecified rows, within bounds).
  * head_dim 256: any window, num_sinks 0..G4_MAX_SINKS with a window; head_dim
  * 512: neither.
  */

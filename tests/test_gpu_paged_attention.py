@@ -81,6 +81,30 @@ def test_hundreds_of_sequences():
     run(5, 256, 1, 2, 32, lens, [1] * 600, 64, 3)
 
 
+# Chunks: more than 64 query rows per KV head are attended over bf16 rows in the workspace.
+@pytest.mark.parametrize("d,hkv,grp,page,lens,new,window,sinks", [
+    (512, 4, 8, 64, [900, 9, 300], [500, 9, 0], 0, 0),
+    (512, 4, 8, 64, [6000, 20], [9, 1], 0, 0),  # a prompt's end and a step in one batch
+    (512, 1, 1, 32, [400], [400], 0, 0),
+    (512, 2, 4, 256, [2100, 700], [150, 33], 0, 0),
+    (256, 16, 2, 64, [3000, 1500], [700, 33], 1024, 4),
+    (256, 2, 2, 64, [3000, 1500, 40], [33, 200, 40], 1024, 0),
+    (256, 2, 8, 32, [900, 70], [200, 70], 100, 32),
+    (256, 4, 2, 128, [500, 77], [60, 33], 64, 17),
+    (256, 1, 4, 64, [333, 1], [40, 1], 0, 0),
+])
+def test_chunks(d, hkv, grp, page, lens, new, window, sinks):
+    assert max(new) * grp > 64
+    run(d + page + sum(lens), d, hkv, grp, page, lens, new, window, sinks)
+    run(d + page + sum(lens), d, hkv, grp, page, lens, new, window, sinks, max_q=max(new) + 40,
+        max_k=max(lens) + 100)
+
+
+def test_chunks_of_hundreds_of_sequences():
+    lens = [(37 * b) % 150 + 40 for b in range(300)]
+    run(16, 256, 1, 2, 32, lens, [33 + b % 7 for b in range(300)], 64, 3)
+
+
 def test_one_long_sequence_among_short_ones():
     run(6, 512, 2, 8, 64, [40, 20000, 7, 300], [1, 1, 1, 1])
 
@@ -93,31 +117,38 @@ def test_large_scores():
     check_attention(q, cache, table, [2000], [1], out, lse)
 
 
-def test_queries_that_see_nothing():
+@pytest.mark.parametrize("more", [2, 100])  # read as they lie, and laid out
+@pytest.mark.parametrize("d,window,sinks", [(256, 0, 0), (256, 16, 2), (512, 0, 0)])
+def test_queries_that_see_nothing(d, window, sinks, more):
     # no tokens at all, and more queries than tokens: 0 and -inf
-    cache, table = filled_cache(9, [3, 40], 2, 32, 256)
-    q = queries(9, 9, 4, 256)
-    out, lse = attend(q, cache, table, [3, 0], [5, 4])
-    assert not out[:2].any() and not out[5:].any()
-    assert lse[:, :2].eq(-torch.inf).all() and lse[:, 5:].eq(-torch.inf).all()
-    check_attention(q[2:5], cache, table[:1], [3], [3], out[2:5], lse[:, 2:5])
+    cache, table = filled_cache(9, [3, 40], 2, 32, d)
+    q = queries(9, more + 7, 4, d)
+    out, lse = attend(q, cache, table, [3, 0], [more + 3, 4], window=window, sinks=sinks)
+    seen = slice(more, more + 3)
+    nothing = torch.ones(more + 7, dtype=torch.bool, device=DEV)
+    nothing[seen] = False
+    assert not out[nothing].any() and lse[:, nothing].eq(-torch.inf).all()
+    check_attention(q[seen], cache, table[:1], [3], [3], out[seen], lse[:, seen], window=window,
+                    sinks=sinks)
 
 
-def test_rows_behind_the_last_sequence_stay():
+@pytest.mark.parametrize("new", [2, 45])
+def test_rows_behind_the_last_sequence_stay(new):
     cache, table = filled_cache(10, [50], 2, 32, 256)
-    q = queries(10, 6, 4, 256)
-    out, lse = g4.paged_cache_attention(q, cache, ints(table), ints([50]), ints([0, 2]),
-                                        max_seqlen_q=2, max_seqlen_k=50)
-    check_attention(q[:2], cache, table, [50], [2], out[:2], lse[:, :2])
-    assert out[2:].isnan().all() and lse[:, 2:].isnan().all()  # (the fixture's fill)
+    q = queries(10, new + 4, 4, 256)
+    out, lse = g4.paged_cache_attention(q, cache, ints(table), ints([50]), ints([0, new]),
+                                        max_seqlen_q=new, max_seqlen_k=50)
+    check_attention(q[:new], cache, table, [50], [new], out[:new], lse[:, :new])
+    assert out[new:].isnan().all() and lse[:, new:].isnan().all()  # (the fixture's fill)
 
 
-def test_what_lies_past_the_end_and_in_other_pages_is_not_seen():
+@pytest.mark.parametrize("new", [[2, 1], [70, 3]])
+def test_what_lies_past_the_end_and_in_other_pages_is_not_seen(new):
     # NaN bytes everywhere but in the tokens: past the last row, in free pages, and in the
     # pages between the sinks and the window, which are gone from the table
-    lens, new, window, sinks = [333, 61], [2, 1], 64, 3
+    lens, window, sinks = [333, 61], 64, 3
     clean, table = filled_cache(11, lens, 2, 32, 256)
-    q = queries(11, 3, 4, 256)
+    q = queries(11, sum(new), 4, 256)
     want = attend(q, clean, table, lens, new, window=window, sinks=sinks)
     cache, _ = filled_cache(11, lens, 2, 32, 256)
     used = torch.zeros(cache.num_pages, 32, dtype=torch.bool)
@@ -147,6 +178,41 @@ def test_a_visible_token_without_a_page_gives_nan(entry):
     got, lse = attend(q, cache, table, lens, new)
     assert got[0].isnan().all() and got[2:].isnan().all()
     assert torch.equal(got[1], want[1]) and torch.equal(lse[:, 1], want_lse[:, 1])
+
+
+@pytest.mark.parametrize("d", [256, 512])
+def test_a_chunk_and_a_token_without_a_page(d):
+    lens, new = [200, 100], [80, 70]
+    cache, table = filled_cache(17, lens, 2, 32, d)
+    q = queries(17, 150, 4, d)
+    want, want_lse = attend(q, cache, table, lens, new)
+    table[0][4] = -1  # tokens 128 .. 159, of the chunk itself: seen from position 128 on
+    got, lse = attend(q, cache, table, lens, new)
+    assert torch.equal(got[:8], want[:8]) and got[8:80].isnan().all()
+    assert torch.equal(got[80:], want[80:]) and torch.equal(lse[:, 80:], want_lse[:, 80:])
+
+
+def test_a_captured_chunk():
+    lens, new = [400, 300], [90, 60]
+    cache, table = filled_cache(18, lens, 2, 64, 256)
+    q = queries(18, 150, 4, 256)
+    tab, ln, cu = ints(table), ints(lens), ints(cu_of(new))
+
+    def call():
+        return g4.paged_cache_attention(q, cache, tab, ln, cu, max_seqlen_q=90, max_seqlen_k=400,
+                                        sliding_window=64, num_sinks=4)
+
+    call()  # (launch attributes are set outside the capture)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(5):
+        q.copy_(queries(40 + i, 150, 4, 256))
+        ln.copy_(ints([400 - 7 * i, 300 - i]))
+        graph.replay()
+        want = call()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check_attention(q, cache, table, [372, 296], new, *got, window=64, sinks=4)
 
 
 def test_a_table_narrower_than_the_lengths():
