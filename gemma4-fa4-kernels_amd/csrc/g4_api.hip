@@ -972,17 +972,20 @@ static g4::CacheAttnParams cache_attn_params(const g4_cache_attn& p) {
   a.max_k = p.max_seqlen_k;
   a.window = p.window;
   a.sinks = p.num_sinks;
-  a.group_queries = 16 / (p.num_q_heads / p.cache.num_kv_heads);
-  a.groups = (p.max_seqlen_q + a.group_queries - 1) / a.group_queries;
   return a;
 }
 
 // Larger chunks of new tokens: the visible rows of every sequence as bf16 in the
 // workspace, and the forward of g4_attn_fwd over them.  Reading pages as they lie
-// costs the whole cache once per group of 16 query rows, the copy five times its
-// bytes once.
+// costs the cache once per 64 query rows of a KV head and a conversion per 16, the
+// copy five times the cache's bytes once, whatever the rows.  As they lie / laid out,
+// us, head dim 512 (8 heads a KV head), by rows: 16 x 8192 tokens 64: 269 / 634, 128:
+// 505 / 644, 192: 756 / 750; 16 x 1000 64: 65 / 87, 128: 130 / 96; 1 x 8192 128: 63 /
+// 86, 256: 83 / 86.  Head dim 256 with a window of 1024: 16 x 8192 128: 112 / 204, 192:
+// 192 / 218; 16 x 1000 192: 183 / 190; 1 x 1000 192: 43 / 50.
 struct CacheExpand {
-  static constexpr int kRows = 64;  // query rows of a KV head from which on it is taken
+  // query rows of a KV head that are read as they lie
+  static int as_they_lie(int head_dim) { return head_dim == 512 ? 128 : 192; }
   static constexpr size_t kMost = size_t(8) << 30;  // bytes of rows at most
   g4_problem p;
   int64_t rows;       // of K and of V in the workspace
@@ -996,7 +999,7 @@ struct CacheExpand {
     rows = most * a.table.batch;
     operand = align256((size_t)rows * hkv * d * 2);
     cu = align256((size_t)(a.table.batch + 1) * 4);
-    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > kRows && 2 * operand <= kMost &&
+    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(d) && 2 * operand <= kMost &&
            rows < 0x7fffffffLL && (int64_t)hkv * d < (int64_t(1) << 24) &&
            (int64_t)a.table.batch * a.max_seqlen_q < 0x7fffffffLL;
     p = g4_problem{};
@@ -1069,8 +1072,7 @@ int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void*
   a.lse = lse;
   a.ql = ql;
   a.ol = ol;
-  a.part = (float*)ws;
-  hipError_t e = g4::launch_cache_attn(a, (hipStream_t)stream);
+  hipError_t e = g4::launch_cache_attn(a, ws, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "cache attention");
   return G4_OK;
 }

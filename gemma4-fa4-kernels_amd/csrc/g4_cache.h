@@ -129,13 +129,15 @@ struct CacheAttnParams {
   __bf16* o;
   float* lse;
   g4_layout ql, ol;
-  float* part;         // partial rows of the segments that several parts share
-  int parts;           // workgroups at most (set by the launcher)
-  int groups;          // row groups of a sequence at most
-  int group_queries;   // queries of a group: 16 / (query heads of a KV head)
+  // Set by the launcher (g4_cache_attn.hip): workgroups at most, groups and queries of
+  // a set, sets of a sequence at most; the parts' heads, and partial rows of the
+  // segments that several parts share.
+  int parts, set_groups, set_queries, sets;
+  struct PartHead* heads;
+  float* part;
 };
-size_t cache_part_bytes(const CacheAttnParams& a);
-hipError_t launch_cache_attn(CacheAttnParams a, hipStream_t stream);
+size_t cache_part_bytes(CacheAttnParams a);
+hipError_t launch_cache_attn(CacheAttnParams a, void* ws, hipStream_t stream);
 
 // A call on the tables; what a call does not use is null or 0.
 struct PagesParams {

@@ -14,12 +14,15 @@
 // conversion applies them), Q stays bf16: the only roundings are P's to bf16 and
 // the output's.
 //
-// The tiles of all (sequence, row group, KV head) segments, in that order, are cut
-// into equal parts, one workgroup of four waves each, so that the longest sequence
-// of a batch does not decide its time.  The waves of a part take every fourth tile
-// of a segment and add up through LDS; a segment inside one part is finished there,
-// else the parts' sums go to the workspace (slot = part + segment: along the parts
-// both only grow, so no two pairs share one) and a second launch merges them.
+// One, two or four groups (a set) share a workgroup of four waves, which then take
+// the set's tiles side by side, so that a tile comes from memory once for up to 64
+// rows.  The tiles of all (sequence, set, KV head) segments, in that order, are cut
+// into equal parts, one workgroup each, so that the longest sequence of a batch
+// does not decide its time.  A group's waves take its tiles in turn and add up
+// through LDS; a segment inside one part is finished there, else the parts' sums go
+// to the workspace (slot = part + segment: along the parts both only grow, so no
+// two pairs share one), and the second launch has a workgroup for each cut: those
+// of one segment share its rows' elements evenly.
 //
 // Bound by HBM for long batches (1 byte an element of K and V), by the chain of
 // launch, table, page and merge latencies for short ones.
@@ -53,9 +56,6 @@ __device__ __forceinline__ float rows_sum(float x) {
 constexpr int kTile = kCacheBlock;  // keys of a tile: one block of a page, one scale
 constexpr int kWaves = 4;
 constexpr int kGroupRows = 16;
-// Tiles a part has at least: one for each of its waves.
-constexpr int kPartTiles = kWaves;
-
 // A sequence of the batch as the kernels see it.
 struct CacheSeq {
   int q0, lq, len;  // first query row, queries, cached tokens
@@ -84,17 +84,21 @@ struct TileRange {
   __device__ __forceinline__ int at(int x) const { return x < nsink ? x : first + x - nsink; }
 };
 
-// Tiles of a sequence's row groups together, over all its KV heads.
-__device__ __forceinline__ int64_t sequence_tiles(const CacheAttnParams& a, int s) {
-  CacheSeq q;
-  q.init(a, s);
+// Tiles of a sequence's sets together, over all its KV heads.
+__device__ __forceinline__ int64_t sequence_tiles(const CacheAttnParams& a, const CacheSeq& q) {
   int64_t n = 0;
-  for (int i = 0; i < q.lq; i += a.group_queries) {
+  for (int i = 0; i < q.lq; i += a.set_queries) {
     TileRange t;
-    t.init(a, q, i, min(i + a.group_queries, q.lq) - 1);
+    t.init(a, q, i, min(i + a.set_queries, q.lq) - 1);
     n += t.n;
   }
   return n * a.c.num_kv_heads;
+}
+
+__device__ __forceinline__ int64_t sequence_tiles(const CacheAttnParams& a, int s) {
+  CacheSeq q;
+  q.init(a, s);
+  return sequence_tiles(a, q);
 }
 
 // Sum of x over the workgroup (256 threads) and the sum before this thread.
@@ -120,28 +124,88 @@ __device__ __forceinline__ int64_t block_before(int64_t x, int64_t G4_LDS* lds, 
   return before;
 }
 
-// Tiles of the whole batch; every thread of the workgroup (256) calls it.
-__device__ __forceinline__ int64_t batch_tiles(const CacheAttnParams& a, int64_t G4_LDS* lds) {
-  int64_t sum = 0;
+// Tile x of the batch's `tiles`: the sequence it belongs to and that sequence's first
+// tile; every thread of the workgroup (256) calls it.  The part is looked up in the
+// same pass: it holds the tiles from tiles part / parts on.  False: no such part.
+// (in scalar registers, which the wave's tiles leave free)
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return ((int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+struct PartStart {
+  int64_t tiles, lo, hi, seq0;
+  int parts, s;
+  CacheSeq seq;  // sequence s
+};
+__device__ __forceinline__ int part_count(const CacheAttnParams& a, int64_t tiles) {
+  // (each of a set's groups has kWaves / sets waves: at least a tile for each)
+  return (int)max(min((int64_t)a.parts, tiles / (kWaves / a.set_groups)), (int64_t)(tiles > 0));
+}
+__device__ __forceinline__ int part_of(int64_t x, int parts, int64_t tiles) {
+  return (int)(((x + 1) * parts - 1) / tiles);
+}
+__device__ __forceinline__ bool find_part(const CacheAttnParams& a, int part, int64_t G4_LDS* lds,
+                                          PartStart& f) {
+  if (a.tab.batch <= 64) {
+    // one sequence a lane, in every wave by itself: no LDS, no barrier
+    const int lane = threadIdx.x & 63;
+    CacheSeq q;
+    q.init(a, min(lane, a.tab.batch - 1));
+    const int64_t n = lane < a.tab.batch ? sequence_tiles(a, q) : 0;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    f.tiles = uniform(__shfl(incl, 63, 64));
+    f.parts = part_count(a, f.tiles);
+    if (part >= f.parts) return false;
+    f.lo = f.tiles * part / f.parts;
+    f.hi = f.tiles * (part + 1) / f.parts;
+    f.s = __builtin_amdgcn_readfirstlane(__popcll(__ballot(incl <= f.lo)));
+    f.seq0 = uniform(__shfl(incl - n, f.s, 64));
+    f.seq.q0 = __builtin_amdgcn_readlane(q.q0, f.s);
+    f.seq.lq = __builtin_amdgcn_readlane(q.lq, f.s);
+    f.seq.len = __builtin_amdgcn_readlane(q.len, f.s);
+    return true;
+  }
+  f.tiles = 0;
   for (int s0 = 0; s0 < a.tab.batch; s0 += 256) {
     const int s = s0 + (int)threadIdx.x;
     int64_t total;
     block_before(s < a.tab.batch ? sequence_tiles(a, s) : 0, lds, total);
-    sum += total;
+    f.tiles = uniform(f.tiles + total);
   }
-  return sum;
-}
-
-// The parts that a batch of `tiles` tiles is cut into, and the part of tile x: part
-// w holds the tiles from tiles w / parts on.
-__device__ __forceinline__ int64_t part_count(const CacheAttnParams& a, int64_t tiles) {
-  return max(min((int64_t)a.parts, tiles / kPartTiles), (int64_t)1);
-}
-__device__ __forceinline__ int64_t part_of(int64_t x, int64_t parts, int64_t tiles) {
-  return ((x + 1) * parts - 1) / tiles;
+  f.parts = part_count(a, f.tiles);
+  if (part >= f.parts) return false;
+  f.lo = f.tiles * part / f.parts;
+  f.hi = f.tiles * (part + 1) / f.parts;
+  int64_t base = 0;
+  for (int s0 = 0; base <= f.lo; s0 += 256) {
+    const int s = s0 + (int)threadIdx.x;
+    const int64_t n = s < a.tab.batch ? sequence_tiles(a, s) : 0;
+    int64_t total;
+    const int64_t before = base + block_before(n, lds, total);
+    if (before <= f.lo && f.lo < before + n) lds[kWaves] = s, lds[kWaves + 1] = before;
+    base += total;
+  }
+  barrier_lds();
+  f.s = __builtin_amdgcn_readfirstlane((int)lds[kWaves]);
+  f.seq0 = uniform(lds[kWaves + 1]);
+  f.seq.init(a, f.s);
+  return true;
 }
 
 }  // namespace
+
+// What a part leaves for the merge: the segment it begins in (its number, first tile,
+// tiles, KV head, first query's row and rows) and the batch's tiles and parts.
+struct PartHead {
+  int64_t tiles, seg0, segment;
+  int parts, n, kvh, q_row, rows, pad;
+};
+static_assert(sizeof(PartHead) == 48, "a part's head");
 
 template <int D>
 struct CacheWave {
@@ -267,56 +331,48 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
   constexpr int kPitch = D + 4;  // floats of a row in LDS
   __shared__ __attribute__((aligned(16))) float rows[kWaves][kGroupRows][kPitch];
   __shared__ float state[2][kWaves][kGroupRows];
-  __shared__ int64_t scan[kWaves];
-  __shared__ int64_t found[2];
-  int64_t G4_LDS* sh = (int64_t G4_LDS*)scan;
+  __shared__ int64_t scan[kWaves + 2];
   const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hkv = a.c.num_kv_heads;
+  const int sets = a.set_groups, turns = kWaves / sets;  // groups of a set, waves of a group
+  const int sub = wave % sets, turn = wave / sets;       // this wave's group and turn
 
   // ---- this part's tiles [lo, hi) and the sequence of the first --------------
-  const int64_t tiles = batch_tiles(a, sh);
-  const int64_t parts = part_count(a, tiles);
-  const int64_t part = blockIdx.x;
-  if (part >= parts || tiles == 0) return;
-  int64_t lo = tiles * part / parts;
-  const int64_t hi = tiles * (part + 1) / parts;
-  int64_t base = 0;
-  int s = 0;
-  for (int s0 = 0; s0 < a.tab.batch; s0 += 256) {
-    const int sx = s0 + tid;
-    const int64_t n = sx < a.tab.batch ? sequence_tiles(a, sx) : 0;
-    int64_t total;
-    const int64_t before = base + block_before(n, sh, total);
-    if (before <= lo && lo < before + n) found[0] = sx, found[1] = before;
-    base += total;
-    if (base > lo) break;
+  const int part = blockIdx.x;
+  PartStart f;
+  if (!find_part(a, part, (int64_t G4_LDS*)scan, f)) {
+    if (part == 0 && tid == 0) a.heads[0].parts = 0;
+    return;
   }
-  __syncthreads();
-  s = __builtin_amdgcn_readfirstlane((int)found[0]);
-  int64_t seg0 = found[1];  // first tile of the segment at hand
-
-  CacheSeq sq;
-  sq.init(a, s);
-  int group = 0, kvh = 0;
-  // the segment of tile lo
+  int64_t lo = f.lo;
+  const int64_t hi = f.hi;
+  int s = f.s;
+  CacheSeq sq = f.seq;
+  int64_t seg0 = f.seq0;  // first tile of the segment at hand
+  int set = 0, kvh = 0;
   TileRange range;
-  for (;; ++group) {
-    range.init(a, sq, group * a.group_queries,
-               min((group + 1) * a.group_queries, sq.lq) - 1);
+  for (;; ++set) {
+    range.init(a, sq, set * a.set_queries, min((set + 1) * a.set_queries, sq.lq) - 1);
     const int64_t n = (int64_t)range.n * hkv;
     if (lo < seg0 + n) break;
     seg0 += n;
   }
   kvh = (int)((lo - seg0) / range.n);
   seg0 += (int64_t)kvh * range.n;
-
   const int grp = a.num_q_heads / hkv, gsh = __builtin_ctz(grp);
+  if (tid == 0)
+    a.heads[part] = PartHead{f.tiles, seg0, ((int64_t)s * a.sets + set) * hkv + kvh, f.parts,
+                             range.n, kvh, sq.q0 + set * a.set_queries,
+                             min(a.set_queries, sq.lq - set * a.set_queries) << gsh, 0};
+  const int blocks = a.c.page_size / kTile;
   while (true) {
     // ---- the part's share [x0, x1) of the segment's tiles ---------------------
     const int x0 = (int)(lo - seg0), x1 = (int)min(hi - seg0, (int64_t)range.n);
-    const int q_first = group * a.group_queries;
-    const int q_last = min(q_first + a.group_queries, sq.lq) - 1;
+    const int set_first = set * a.set_queries;
+    const int set_last = min(set_first + a.set_queries, sq.lq) - 1;
+    const int q_first = set_first + sub * (kGroupRows >> gsh);  // of this wave's group
+    const int q_last = min(q_first + (kGroupRows >> gsh) - 1, set_last);
     const int off = sq.len - sq.lq;
     const int my_q = q_first + (i >> gsh);
     const int head = kvh * grp + (i & (grp - 1));
@@ -326,7 +382,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
 
     W w;
     {
-      const __bf16* qrow = a.q + (int64_t)(sq.q0 + (valid ? my_q : q_first)) * a.ql.token_stride +
+      // (rows past the group's queries: the set's first, whose results are dropped)
+      const __bf16* qrow = a.q + (int64_t)(sq.q0 + (valid ? my_q : set_first)) * a.ql.token_stride +
                            (int64_t)head * a.ql.head_stride + 16 * h;
 #pragma unroll
       for (int c = 0; c < W::kNC; ++c)
@@ -343,11 +400,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
       const int id = at < a.tab.width ? __builtin_amdgcn_readfirstlane(pages[at]) : -1;
       return (unsigned)id < (unsigned)a.c.num_pages ? (int64_t)id * hkv + kvh : -1;
     };
-    const int blocks = a.c.page_size / kTile;
-    int x = x0 + wave;
+    const int end = q_first > q_last ? x0 : x1;  // (a group without queries has no tiles)
+    int x = x0 + turn;
     int t = 0;
     int64_t ph = -1;
-    if (x < x1) {
+    if (x < end) {
       t = range.at(x);
       ph = page_head(t);
       if (ph >= 0) {
@@ -355,13 +412,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
         w.load_v(a, ph, t % blocks, i, h);
       }
     }
-    while (x < x1) {
+    while (x < end) {
       const int kb0 = t * kTile;
       const bool page = ph >= 0;
-      const int xn = x + kWaves;
+      const int xn = x + turns;
       int tn = 0;
       int64_t phn = -1;
-      if (xn < x1) {
+      if (xn < end) {
         tn = range.at(xn);
         phn = page_head(tn);
       }
@@ -402,26 +459,24 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
             f32x4{w.o[b][r], w.o[b + 1][r], w.o[b + 2][r], w.o[b + 3][r]};
     barrier_lds();
     const bool whole = x0 == 0 && x1 == range.n;
-    const int nrows = (q_last - q_first + 1) << gsh;
-    const int64_t segment = ((int64_t)s * a.groups + group) * hkv + kvh;
-    float* const part_o = a.part + (part + segment) * kGroupRows * (D + 2);
+    const int nrows = (set_last - set_first + 1) << gsh;
+    const int64_t segment = ((int64_t)s * a.sets + set) * hkv + kvh;
+    float* const part_o = a.part + (part + segment) * (int64_t)(sets * kGroupRows * (D + 2));
     constexpr int kCols = D / 4;  // threads of a row, four elements each
     for (int r = tid / kCols; r < nrows; r += 256 / kCols) {
-      const int d = tid % kCols * 4;
-      float mx = state[0][0][r];
-#pragma unroll
-      for (int u = 1; u < kWaves; ++u) mx = fmaxf(mx, state[0][u][r]);
+      const int d = tid % kCols * 4, g = r / kGroupRows, ri = r % kGroupRows;
+      float mx = kNegInf;
+      for (int u = g; u < kWaves; u += sets) mx = fmaxf(mx, state[0][u][ri]);
       const float m_use = mx == kNegInf ? 0.f : mx;
       float sum = 0.f;
       f32x4 acc = {};
-#pragma unroll
-      for (int u = 0; u < kWaves; ++u) {
-        const float wt = fast_exp2(state[0][u][r] - m_use);
-        sum += wt * state[1][u][r];
-        acc += wt * *(const f32x4*)&rows[u][r][d];
+      for (int u = g; u < kWaves; u += sets) {
+        const float wt = fast_exp2(state[0][u][ri] - m_use);
+        sum += wt * state[1][u][ri];
+        acc += wt * *(const f32x4*)&rows[u][ri][d];
       }
       if (whole) {
-        const int qi = q_first + (r >> gsh), qh = kvh * grp + (r & (grp - 1));
+        const int qi = set_first + (r >> gsh), qh = kvh * grp + (r & (grp - 1));
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays)
         *(bf16x4*)(a.o + (int64_t)(sq.q0 + qi) * a.ol.token_stride +
                    (int64_t)qh * a.ol.head_stride + d) =
@@ -433,8 +488,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
       } else {
         *(f32x4*)(part_o + r * D + d) = acc;
         if (d == 0) {
-          part_o[kGroupRows * D + 2 * r] = mx;
-          part_o[kGroupRows * D + 2 * r + 1] = sum;
+          float* const ml = part_o + sets * kGroupRows * D + 2 * r;
+          ml[0] = mx;
+          ml[1] = sum;
         }
       }
     }
@@ -445,102 +501,109 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
     seg0 = lo;
     if (++kvh == hkv) {
       kvh = 0;
-      ++group;
-      while (group * a.group_queries >= sq.lq) {  // (tiles are left, so sequences are)
+      ++set;
+      while (set * a.set_queries >= sq.lq) {  // (tiles are left, so sequences are)
         sq.init(a, ++s);
-        group = 0;
+        set = 0;
       }
-      range.init(a, sq, group * a.group_queries,
-                 min((group + 1) * a.group_queries, sq.lq) - 1);
+      range.init(a, sq, set * a.set_queries, min((set + 1) * a.set_queries, sq.lq) - 1);
     }
   }
 }
 
-// O and LSE of the segments that more than one part holds.  One workgroup per
-// (segment, row, SPLIT-th of the head dim).
-template <int D, int SPLIT>
+// O and LSE of the segments that more than one part holds.  The workgroup of part w
+// serves the segment that part w begins inside of, as one of the n - 1 workgroups
+// whose parts do: each takes an equal run of the rows' elements, four a thread, and
+// where those are fewer than the threads, several threads share the parts.
+template <int D>
 __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
-  constexpr int kCols = D / SPLIT / 4;  // threads of a row, four elements each
-  constexpr int kSubs = 256 / kCols;    // parts added side by side
-  __shared__ int64_t scan[kWaves];
-  __shared__ float red[2][kWaves];
-  __shared__ __attribute__((aligned(16))) float stage[kSubs][D / SPLIT];
-  int64_t G4_LDS* sh = (int64_t G4_LDS*)scan;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hkv = a.c.num_kv_heads;
-  const int split = blockIdx.y, row = blockIdx.x % kGroupRows;
-  const int64_t segment = blockIdx.x / kGroupRows;
-  const int kvh = (int)(segment % hkv), group = (int)(segment / hkv % a.groups);
-  const int s = (int)(segment / hkv / a.groups);
-  const int grp = a.num_q_heads / hkv, gsh = __builtin_ctz(grp);
-  CacheSeq sq;
-  sq.init(a, s);
-  const int qi = group * a.group_queries + (row >> gsh), qh = kvh * grp + (row & (grp - 1));
-  if (row >= a.group_queries << gsh || qi >= sq.lq) return;
+  __shared__ __attribute__((aligned(16))) float acc_lds[256][4];
+  __shared__ float ml_lds[256][2];
+  const int w = blockIdx.x + 1, tid = threadIdx.x;
+  const PartHead& first = a.heads[0];
+  const PartHead hd = a.heads[w];
+  const int parts = first.parts;
+  if (w >= parts) return;
+  const int64_t tiles = first.tiles;
+  if (tiles * w / parts == hd.seg0) return;  // begins with the segment
+  const int w0 = part_of(hd.seg0, parts, tiles);
+  const int n = part_of(hd.seg0 + hd.n - 1, parts, tiles) - w0 + 1;
 
-  // ---- the parts that hold the segment -----------------------------------------
-  int64_t tiles = 0, first = 0;
-  for (int s0 = 0; s0 < a.tab.batch; s0 += 256) {
-    const int sx = s0 + tid;
-    const int64_t n = sx < a.tab.batch ? sequence_tiles(a, sx) : 0;
-    int64_t total, mine;
-    block_before(n, sh, total);
-    tiles += total;
-    block_before(sx < s ? n : 0, sh, mine);
-    first += mine;
-  }
-  TileRange range;
-  for (int g = 0; g <= group; ++g) {
-    range.init(a, sq, g * a.group_queries, min((g + 1) * a.group_queries, sq.lq) - 1);
-    first += (int64_t)range.n * (g < group ? hkv : kvh);
-  }
-  const int64_t parts = part_count(a, tiles);
-  const int64_t w0 = part_of(first, parts, tiles);
-  const int n = (int)(part_of(first + range.n - 1, parts, tiles) - w0) + 1;
-  if (n == 1) return;  // finished by its one part
+  const int grp = a.num_q_heads / a.c.num_kv_heads, gsh = __builtin_ctz(grp);
+  const int set_rows = a.set_groups * kGroupRows;
+  const int64_t slot = (int64_t)set_rows * (D + 2);
+  const float* const part = a.part + (w0 + hd.segment) * slot;
 
-  // ---- weights 2^(m_c - M), then the rows -----------------------------------------
-  constexpr int64_t kSlot = kGroupRows * (D + 2);
-  const float* const part = a.part + (w0 + segment) * kSlot;
-  const float* const ml = part + kGroupRows * D + 2 * row;
-  float mx = kNegInf;
-  for (int c = tid; c < n; c += 256) mx = fmaxf(mx, ml[c * kSlot]);
+  const int units = hd.rows * (D / 4);  // four elements of a row each
+  const int u0 = (int)((int64_t)units * (w - w0 - 1) / (n - 1));
+  const int u1 = (int)((int64_t)units * (w - w0) / (n - 1));
+  int subs = 1;  // threads of a unit
+  while (subs < 16 && subs * 2 * (u1 - u0) <= 256) subs *= 2;
+  const int per = 256 / subs;
+  for (int ub = u0; ub < u1; ub += per) {
+    const int u = ub + tid / subs, sub = tid % subs;
+    const bool mine = u < u1;
+    const int r = mine ? u / (D / 4) : 0, d = u % (D / 4) * 4;
+    const float* const ml = part + set_rows * D + 2 * r;
+    const float* const po = part + r * D + d;
+    float mx = kNegInf, sum = 0.f;
+    f32x4 acc = {};
+    if (mine) {
+      // four parts at a time, their loads in flight together
+      for (int c0 = sub; c0 < n; c0 += 4 * subs) {
+        f32x2 ml4[4];
+        f32x4 o4[4];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  if (lane == 0) red[0][wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float m_use = mx == kNegInf ? 0.f : mx;
-  const int sub = tid / kCols, d = tid % kCols * 4;
-  const float* const po = part + row * D + split * (D / SPLIT) + d;
-  f32x4 acc = {};
-  float sum = 0.f;
-#pragma unroll 4
-  for (int c = sub; c < n; c += kSubs) {
-    const float wt = fast_exp2(ml[c * kSlot] - m_use);
-    sum += wt * ml[c * kSlot + 1];
-    acc += wt * *(const f32x4*)(po + c * kSlot);
-  }
-  *(f32x4*)&stage[sub][d] = acc;
-  // (each column's thread holds its sub's share of the sum)
-  __shared__ float sums[kSubs];
-  if (d == 0) sums[sub] = sum;
-  __syncthreads();
-  if (sub != 0) return;
-  acc = f32x4{};
-  sum = 0.f;
+        for (int v = 0; v < 4; ++v) {
+          const int c = min(c0 + v * subs, n - 1);
+          ml4[v] = *(const f32x2*)(ml + c * slot);
+          o4[v] = *(const f32x4*)(po + c * slot);
+        }
+        float m_new = mx;
 #pragma unroll
-  for (int u = 0; u < kSubs; ++u) {
-    acc += *(const f32x4*)&stage[u][d];
-    sum += sums[u];
+        for (int v = 0; v < 4; ++v)
+          if (c0 + v * subs < n) m_new = fmaxf(m_new, ml4[v][0]);
+        const float m_use = m_new == kNegInf ? 0.f : m_new;
+        const float alpha = fast_exp2(mx - m_use);
+        sum *= alpha;
+        acc *= alpha;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (c0 + v * subs < n) {
+            const float wt = fast_exp2(ml4[v][0] - m_use);
+            sum += wt * ml4[v][1];
+            acc += wt * o4[v];
+          }
+        mx = m_new;
+      }
+    }
+    if (subs > 1) {
+      __syncthreads();
+      *(f32x4*)acc_lds[tid] = acc;
+      ml_lds[tid][0] = mx;
+      ml_lds[tid][1] = sum;
+      __syncthreads();
+      if (sub != 0) continue;
+      for (int v = 1; v < subs; ++v) mx = fmaxf(mx, ml_lds[tid + v][0]);
+      const float m_use = mx == kNegInf ? 0.f : mx;
+      sum = 0.f;
+      acc = f32x4{};
+      for (int v = 0; v < subs; ++v) {
+        const float wt = fast_exp2(ml_lds[tid + v][0] - m_use);
+        sum += wt * ml_lds[tid + v][1];
+        acc += wt * *(const f32x4*)acc_lds[tid + v];
+      }
+    }
+    if (!mine) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int qrow = hd.q_row + (r >> gsh), qh = hd.kvh * grp + (r & (grp - 1));
+    *(bf16x4*)(a.o + (int64_t)qrow * a.ol.token_stride + (int64_t)qh * a.ol.head_stride +
+               d) = bf16x4{(__bf16)(acc[0] * inv), (__bf16)(acc[1] * inv),
+                           (__bf16)(acc[2] * inv), (__bf16)(acc[3] * inv)};
+    if (d == 0)
+      a.lse[(int64_t)qh * a.total_q + qrow] =
+          sum == 0.f ? kNegInf : (mx + fast_log2(sum)) * kLn2;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *(bf16x4*)(a.o + (int64_t)(sq.q0 + qi) * a.ol.token_stride + (int64_t)qh * a.ol.head_stride +
-             split * (D / SPLIT) + d) = bf16x4{(__bf16)(acc[0] * inv), (__bf16)(acc[1] * inv),
-                                               (__bf16)(acc[2] * inv), (__bf16)(acc[3] * inv)};
-  if (split == 0 && d == 0)
-    a.lse[(int64_t)qh * a.total_q + sq.q0 + qi] =
-        sum == 0.f ? kNegInf : (mx + fast_log2(sum)) * kLn2;
 }
 
 // ---- launches -------------------------------------------------------------------
@@ -549,12 +612,27 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
 static int cache_parts(int head_dim) { return head_dim == 256 ? 512 : 256; }
 
 static int64_t cache_segments(const CacheAttnParams& a) {
-  return (int64_t)a.tab.batch * a.groups * a.c.num_kv_heads;
+  return (int64_t)a.tab.batch * a.sets * a.c.num_kv_heads;
 }
 
-size_t cache_part_bytes(const CacheAttnParams& a) {
-  const int64_t slots = cache_parts(a.c.head_dim) + cache_segments(a);
-  return (size_t)slots * kGroupRows * (a.c.head_dim + 2) * 4;
+// Groups of a set: as many as the batch's longest run of new tokens fills.
+static void cache_sets(CacheAttnParams* a) {
+  const int grp = a->num_q_heads / a->c.num_kv_heads;
+  const int64_t rows = (int64_t)a->max_q * grp;
+  a->set_groups = rows <= kGroupRows ? 1 : rows <= 2 * kGroupRows ? 2 : 4;
+  a->set_queries = a->set_groups * kGroupRows / grp;
+  a->sets = (a->max_q + a->set_queries - 1) / a->set_queries;
+  a->parts = cache_parts(a->c.head_dim);
+}
+
+static size_t heads_bytes(const CacheAttnParams& a) {
+  return ((size_t)a.parts * sizeof(PartHead) + 255) & ~size_t(255);
+}
+
+size_t cache_part_bytes(CacheAttnParams a) {
+  cache_sets(&a);
+  const int64_t slots = a.parts + cache_segments(a);
+  return heads_bytes(a) + (size_t)slots * a.set_groups * kGroupRows * (a.c.head_dim + 2) * 4;
 }
 
 template <int D>
@@ -562,13 +640,14 @@ static hipError_t launch_cache_attn_d(const CacheAttnParams& a, hipStream_t stre
   hipLaunchKernelGGL(cache_attn_kernel<D>, dim3((unsigned)a.parts), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned rows = (unsigned)(cache_segments(a) * kGroupRows);
-  hipLaunchKernelGGL((cache_merge_kernel<D, 4>), dim3(rows, 4), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(cache_merge_kernel<D>, dim3((unsigned)a.parts - 1), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
-hipError_t launch_cache_attn(CacheAttnParams a, hipStream_t stream) {
-  a.parts = cache_parts(a.c.head_dim);
+hipError_t launch_cache_attn(CacheAttnParams a, void* ws, hipStream_t stream) {
+  cache_sets(&a);
+  a.heads = (PartHead*)ws;
+  a.part = (float*)((char*)ws + heads_bytes(a));
   return a.c.head_dim == 256 ? launch_cache_attn_d<256>(a, stream)
                              : launch_cache_attn_d<512>(a, stream);
 }

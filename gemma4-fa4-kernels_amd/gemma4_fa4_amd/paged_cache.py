@@ -221,7 +221,7 @@ def paged_cache_attention(
     window nor sinks; query heads are 1, 2, 4 or 8 times the cache's.
 
     A few new tokens per sequence are computed from the pages as they lie; from more
-    than 64 query rows per KV head on, what the batch can see is laid out as bf16 rows
+    than 128 query rows per KV head on (192 at head dim 256), what the batch can see is laid out as bf16 rows
     in a workspace (``4 * batch * tokens * Hkv * head_dim`` bytes, up to 8 GiB).
     """
     if q.ndim != 3 or q.dtype != torch.bfloat16:

@@ -33,7 +33,11 @@ def run(seed, d, hkv, grp, page, lens, new, window=0, sinks=0, **kw):
     (512, 2, 1, 128, [100, 257], [1, 1]),  # GQA 1
     (512, 1, 2, 64, [300], [8]),  # a whole group of 16 rows
     (512, 1, 4, 64, [300, 90], [7, 3]),  # two groups, the second part full
-    (512, 4, 8, 64, [515, 12, 200], [5, 0, 12]),  # three groups, none, six
+    (512, 4, 8, 64, [515, 12, 200], [5, 0, 8]),  # three groups, none, a set of four
+    (512, 2, 8, 64, [4000, 33, 7], [3, 4, 1]),  # sets of two, one group of one empty
+    (512, 2, 4, 32, [2000, 3, 90, 77], [16, 3, 9, 1]),
+    (256, 2, 1, 64, [900, 64], [64, 20]),
+    (256, 2, 8, 128, [300, 1, 40], [4, 1, 2]),
     (256, 16, 2, 64, [900], [1]),
     (256, 3, 2, 32, [130, 1, 500], [3, 1, 17]),
     (256, 2, 8, 128, [77, 40], [40, 40]),
@@ -81,20 +85,24 @@ def test_hundreds_of_sequences():
     run(5, 256, 1, 2, 32, lens, [1] * 600, 64, 3)
 
 
-# Chunks: more than 64 query rows per KV head are attended over bf16 rows in the workspace.
+# Chunks: more than 128 query rows per KV head (192 at head dim 256) are attended over bf16
+# rows in the workspace; shorter ones of these in several sets of rows.
 @pytest.mark.parametrize("d,hkv,grp,page,lens,new,window,sinks", [
     (512, 4, 8, 64, [900, 9, 300], [500, 9, 0], 0, 0),
-    (512, 4, 8, 64, [6000, 20], [9, 1], 0, 0),  # a prompt's end and a step in one batch
+    (512, 4, 8, 64, [6000, 20], [17, 1], 0, 0),  # a prompt's end and a step in one batch
+    (512, 4, 8, 64, [600, 20, 50], [16, 1, 9], 0, 0),  # two sets
     (512, 1, 1, 32, [400], [400], 0, 0),
+    (256, 1, 1, 32, [400, 193], [400, 193], 100, 3),
     (512, 2, 4, 256, [2100, 700], [150, 33], 0, 0),
     (256, 16, 2, 64, [3000, 1500], [700, 33], 1024, 4),
     (256, 2, 2, 64, [3000, 1500, 40], [33, 200, 40], 1024, 0),
+    (256, 2, 2, 64, [3000, 1500, 40], [33, 90, 40], 1024, 5),
     (256, 2, 8, 32, [900, 70], [200, 70], 100, 32),
     (256, 4, 2, 128, [500, 77], [60, 33], 64, 17),
+    (256, 4, 2, 128, [500, 77], [97, 33], 64, 17),
     (256, 1, 4, 64, [333, 1], [40, 1], 0, 0),
 ])
 def test_chunks(d, hkv, grp, page, lens, new, window, sinks):
-    assert max(new) * grp > 64
     run(d + page + sum(lens), d, hkv, grp, page, lens, new, window, sinks)
     run(d + page + sum(lens), d, hkv, grp, page, lens, new, window, sinks, max_q=max(new) + 40,
         max_k=max(lens) + 100)
@@ -102,7 +110,7 @@ def test_chunks(d, hkv, grp, page, lens, new, window, sinks):
 
 def test_chunks_of_hundreds_of_sequences():
     lens = [(37 * b) % 150 + 40 for b in range(300)]
-    run(16, 256, 1, 2, 32, lens, [33 + b % 7 for b in range(300)], 64, 3)
+    run(16, 256, 1, 8, 32, lens, [33 + b % 7 for b in range(300)], 64, 3)
 
 
 def test_one_long_sequence_among_short_ones():
@@ -122,7 +130,7 @@ def test_large_scores():
 def test_queries_that_see_nothing(d, window, sinks, more):
     # no tokens at all, and more queries than tokens: 0 and -inf
     cache, table = filled_cache(9, [3, 40], 2, 32, d)
-    q = queries(9, more + 7, 4, d)
+    q = queries(9, more + 7, 8, d)
     out, lse = attend(q, cache, table, [3, 0], [more + 3, 4], window=window, sinks=sinks)
     seen = slice(more, more + 3)
     nothing = torch.ones(more + 7, dtype=torch.bool, device=DEV)
@@ -135,7 +143,7 @@ def test_queries_that_see_nothing(d, window, sinks, more):
 @pytest.mark.parametrize("new", [2, 45])
 def test_rows_behind_the_last_sequence_stay(new):
     cache, table = filled_cache(10, [50], 2, 32, 256)
-    q = queries(10, new + 4, 4, 256)
+    q = queries(10, new + 4, 16, 256)
     out, lse = g4.paged_cache_attention(q, cache, ints(table), ints([50]), ints([0, new]),
                                         max_seqlen_q=new, max_seqlen_k=50)
     check_attention(q[:new], cache, table, [50], [new], out[:new], lse[:, :new])
@@ -148,7 +156,7 @@ def test_what_lies_past_the_end_and_in_other_pages_is_not_seen(new):
     # pages between the sinks and the window, which are gone from the table
     lens, window, sinks = [333, 61], 64, 3
     clean, table = filled_cache(11, lens, 2, 32, 256)
-    q = queries(11, sum(new), 4, 256)
+    q = queries(11, sum(new), 8, 256)
     want = attend(q, clean, table, lens, new, window=window, sinks=sinks)
     cache, _ = filled_cache(11, lens, 2, 32, 256)
     used = torch.zeros(cache.num_pages, 32, dtype=torch.bool)
@@ -184,7 +192,7 @@ def test_a_visible_token_without_a_page_gives_nan(entry):
 def test_a_chunk_and_a_token_without_a_page(d):
     lens, new = [200, 100], [80, 70]
     cache, table = filled_cache(17, lens, 2, 32, d)
-    q = queries(17, 150, 4, d)
+    q = queries(17, 150, 8, d)
     want, want_lse = attend(q, cache, table, lens, new)
     table[0][4] = -1  # tokens 128 .. 159, of the chunk itself: seen from position 128 on
     got, lse = attend(q, cache, table, lens, new)
@@ -195,7 +203,7 @@ def test_a_chunk_and_a_token_without_a_page(d):
 def test_a_captured_chunk():
     lens, new = [400, 300], [90, 60]
     cache, table = filled_cache(18, lens, 2, 64, 256)
-    q = queries(18, 150, 4, 256)
+    q = queries(18, 150, 8, 256)
     tab, ln, cu = ints(table), ints(lens), ints(cu_of(new))
 
     def call():
@@ -207,7 +215,7 @@ def test_a_captured_chunk():
     with torch.cuda.graph(graph):
         got = call()
     for i in range(5):
-        q.copy_(queries(40 + i, 150, 4, 256))
+        q.copy_(queries(40 + i, 150, 8, 256))
         ln.copy_(ints([400 - 7 * i, 300 - i]))
         graph.replay()
         want = call()
