@@ -910,6 +910,12 @@ static int check_rows(const int32_t* cu, int64_t total) {
     return fail(G4_ERR_INVALID, "the number of packed rows must be in [0, 2^31)");
   return G4_OK;
 }
+// Workgroups of an append or a gather: one per 32 rows of a sequence and head.
+static int check_blocks(const g4_paged_cache* c, const g4_page_table* t, int64_t total) {
+  if ((total / 32 + 2 * (int64_t)t->batch) * c->num_kv_heads > 0x7fffffffLL)
+    return fail(G4_ERR_UNSUPPORTED, "rows x heads of one call exceed what a launch covers");
+  return G4_OK;
+}
 
 int g4_cache_append(const g4_paged_cache* cache, const g4_page_table* table, const int32_t* cu,
                     int64_t total, const void* k, g4_layout kl, const void* v, g4_layout vl,
@@ -919,6 +925,7 @@ int g4_cache_append(const g4_paged_cache* cache, const g4_page_table* table, con
   G4_TRY(check_table(table));
   G4_TRY(check_rows(cu, total));
   if (total == 0) return G4_OK;
+  G4_TRY(check_blocks(cache, table, total));
   G4_TRY(check_operand(k, kl, "k"));
   G4_TRY(check_operand(v, vl, "v"));
   g4::AppendParams a{*cache, *table, cu, total, {(const __bf16*)k, (const __bf16*)v}, {kl, vl}};
@@ -934,6 +941,7 @@ int g4_cache_gather(const g4_paged_cache* cache, const g4_page_table* table, con
   G4_TRY(check_table(table));
   G4_TRY(check_rows(cu, total));
   if (total == 0) return G4_OK;
+  G4_TRY(check_blocks(cache, table, total));
   G4_TRY(check_operand(k, kl, "k"));
   G4_TRY(check_operand(v, vl, "v"));
   g4::GatherParams a{*cache, *table, cu, total, {(__bf16*)k, (__bf16*)v}, {kl, vl}};
@@ -1000,7 +1008,7 @@ struct CacheExpand {
     operand = align256((size_t)rows * hkv * d * 2);
     cu = align256((size_t)(a.table.batch + 1) * 4);
     used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(d) && 2 * operand <= kMost &&
-           rows < 0x7fffffffLL && (int64_t)hkv * d < (int64_t(1) << 24) &&
+           (rows / 32 + a.table.batch) * hkv < 0x7fffffffLL && (int64_t)hkv * d < (int64_t(1) << 24) &&
            (int64_t)a.table.batch * a.max_seqlen_q < 0x7fffffffLL;
     p = g4_problem{};
     p.num_seqs = a.table.batch;

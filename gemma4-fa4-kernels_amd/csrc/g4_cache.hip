@@ -21,7 +21,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
   constexpr int kPasses = kCacheBlock / kRows;
   __shared__ int wave_max[4];
   const g4_paged_cache& c = a.c;
-  const int slot = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
+  // heads first: neighbouring workgroups read neighbouring runs of the same rows
+  const int head = blockIdx.x % c.num_kv_heads, slot = blockIdx.x / c.num_kv_heads;
+  const int which = blockIdx.y;
   const int s = find_sequence(a.cu, a.tab.batch, slot, 2);
   const int row0 = a.cu[s], n = a.cu[s + 1] - row0;
   const int len = a.tab.seq_lens[s];
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
 hipError_t launch_cache_append(const AppendParams& a, hipStream_t stream) {
   // a sequence's n new tokens touch at most n / 32 + 2 blocks
   const int64_t slots = a.total / kCacheBlock + 2 * (int64_t)a.tab.batch;
-  const dim3 grid((unsigned)slots, (unsigned)a.c.num_kv_heads, 2);
+  const dim3 grid((unsigned)(slots * a.c.num_kv_heads), 2);
   if (a.c.head_dim == 256)
     hipLaunchKernelGGL(append_kernel<256>, grid, dim3(256), 0, stream, a);
   else
@@ -122,7 +124,8 @@ __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {
   constexpr int kLanes = D / 8;
   constexpr int kRows = 256 / kLanes;
   const g4_paged_cache& c = a.c;
-  const int slot = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
+  const int head = blockIdx.x % c.num_kv_heads, slot = blockIdx.x / c.num_kv_heads;
+  const int which = blockIdx.y;
   const int s = find_sequence(a.cu, a.tab.batch, slot, 1);
   const int row0 = a.cu[s], n = a.cu[s + 1] - row0;
   const int rel = slot - (row0 / 32 + s);
@@ -204,7 +207,7 @@ hipError_t launch_cache_expand_lengths(const ExpandParams& a, hipStream_t stream
 
 hipError_t launch_cache_gather(const GatherParams& a, hipStream_t stream) {
   const int64_t slots = a.total / 32 + a.tab.batch;
-  const dim3 grid((unsigned)slots, (unsigned)a.c.num_kv_heads, 2);
+  const dim3 grid((unsigned)(slots * a.c.num_kv_heads), 2);
   if (a.c.head_dim == 256)
     hipLaunchKernelGGL(gather_kernel<256>, grid, dim3(256), 0, stream, a);
   else

@@ -76,6 +76,7 @@ SHAPES = [  # seed, batch, width, pages, page size
     (4, 70, 4, 200, 128),
     (5, 33, 40, 9000, 32),  # several rounds of the ordering workgroup's scans
     (6, 1500, 3, 5000, 256),  # more rows than its threads
+    (7, 300, 60, 40000, 32),  # more entries than one workgroup forks; scans of several steps
 ]
 
 
@@ -114,9 +115,10 @@ def test_nothing_free_and_nothing_asked():
     pool.compact()
 
 
-def test_entries_that_are_no_pages():
+@pytest.mark.parametrize("entry", [-7, -2])
+def test_entries_that_are_no_pages(entry):
     # tables with IDs out of range: counts of pages are left alone, nothing else is touched
-    table, lens, refs = [[9, -7, 1], [2147483647, 0, -1]], [96, 64], [1, 1, 0, 0]
+    table, lens, refs = [[9, entry, 1], [2147483647, 0, -1]], [96, 64], [1, 1, 0, 0]
     t, l, r = ints(table), ints(lens), ints(refs)
     guard = torch.full((8,), 7, dtype=torch.int32, device=DEV)
     g4.fork_pages(t, l, r, ints([0, 0]), page_size=32)
