@@ -894,8 +894,8 @@ static int check_cache(const g4_paged_cache* c) {
     return fail(G4_ERR_UNSUPPORTED, "cache head_dim must be 256 or 512");
   if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
     return fail(G4_ERR_UNSUPPORTED, "cache page_size must be 32, 64, 128 or 256");
-  if (c->num_pages < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 65535)
-    return fail(G4_ERR_INVALID, "num_pages and num_kv_heads must be positive (heads below 65536)");
+  if (c->num_pages < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 4096)
+    return fail(G4_ERR_INVALID, "num_pages and num_kv_heads must be positive (heads up to 4096)");
   if (c->k == nullptr || c->v == nullptr || ((uintptr_t)c->k) % 16 || ((uintptr_t)c->v) % 16)
     return fail(G4_ERR_INVALID, "cache k and v must be 16-byte aligned");
   if (c->k_scale == nullptr || c->v_scale == nullptr || ((uintptr_t)c->k_scale) % 4 ||
@@ -1001,12 +1001,13 @@ static g4::CacheAttnParams cache_attn_params(const g4_cache_attn& p) {
 // 505 / 644, 192: 756 / 750; 16 x 1000 64: 65 / 87, 128: 130 / 96; 1 x 8192 128: 63 /
 // 86, 256: 83 / 86.  Head dim 256 with a window of 1024: 16 x 8192 128: 112 / 204, 192:
 // 192 / 218; 16 x 1000 192: 183 / 190; 1 x 1000 192: 43 / 50.
+// Sequences are taken as many at a time as fit kMost bytes, at least one.
 struct CacheExpand {
   // query rows of a KV head that are read as they lie
   static int as_they_lie(int head_dim) { return head_dim == 512 ? 128 : 192; }
-  static constexpr size_t kMost = size_t(8) << 30;  // bytes of rows at most
-  g4_problem p;
-  int64_t rows;       // of K and of V in the workspace
+  static constexpr int64_t kMost = int64_t(8) << 30;  // bytes of rows
+  g4_problem p;             // of a step
+  int per;                  // sequences of a step
   size_t cu, operand, fwd;  // bytes of the lengths, of K or V, of the forward's workspace
   bool used;
   explicit CacheExpand(const g4_cache_attn& a) {
@@ -1014,22 +1015,24 @@ struct CacheExpand {
     const int64_t see = a.window > 0 ? (int64_t)a.window + a.max_seqlen_q + a.num_sinks
                                      : (int64_t)a.max_seqlen_k;
     const int64_t most = std::min<int64_t>(a.max_seqlen_k, see);
-    rows = most * a.table.batch;
-    operand = align256((size_t)rows * hkv * d * 2);
-    cu = align256((size_t)(a.table.batch + 1) * 4);
-    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(d) && 2 * operand <= kMost &&
-           (rows / 32 + a.table.batch) * hkv < 0x7fffffffLL && (int64_t)hkv * d < (int64_t(1) << 24) &&
-           (int64_t)a.table.batch * a.max_seqlen_q < 0x7fffffffLL;
+    const int64_t one = most * hkv * d * 4;  // K and V of a sequence
+    const int64_t fit = std::min(kMost / one, (int64_t)0x7fffffff / std::max<int64_t>(most, a.max_seqlen_q));
+    per = (int)std::min<int64_t>(a.table.batch, std::max<int64_t>(1, fit));
+    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(d) &&
+           (int64_t)hkv * d < (int64_t(1) << 24) &&
+           (most * per / 32 + per) * hkv <= 0x7fffffffLL;
+    operand = align256((size_t)most * per * hkv * d * 2);
+    cu = align256((size_t)(per + 1) * 4);
     p = g4_problem{};
-    p.num_seqs = a.table.batch;
+    p.num_seqs = per;
     p.seqlen_q = a.max_seqlen_q;
     p.seqlen_k = (int32_t)most;
     p.num_q_heads = a.num_q_heads;
     p.num_kv_heads = hkv;
     p.head_dim = d;
     p.window = a.window;
-    p.total_q = a.total_q;
-    p.total_k = rows;
+    p.total_q = std::min<int64_t>(a.total_q, (int64_t)per * a.max_seqlen_q);
+    p.total_k = most * per;
     p.lse_head_stride = a.total_q;
     fwd = 0;
     if (used)
@@ -1038,11 +1041,19 @@ struct CacheExpand {
   size_t bytes() const { return 2 * cu + 2 * operand + fwd; }
 };
 
+// A call's problem with its bounds no larger than its rows make them.
+static g4_cache_attn cache_attn_bounded(const g4_cache_attn& p) {
+  g4_cache_attn b = p;
+  b.max_seqlen_q = (int32_t)std::min<int64_t>(p.max_seqlen_q, std::max<int64_t>(p.total_q, 1));
+  return b;
+}
+
 size_t g4_cache_attn_workspace_bytes(const g4_cache_attn* p) {
   g_last_error.clear();
   if (check_cache_attn(p) != G4_OK) return 0;
-  const CacheExpand x(*p);
-  return x.used ? x.bytes() : align256(g4::cache_part_bytes(cache_attn_params(*p)));
+  const g4_cache_attn b = cache_attn_bounded(*p);
+  const CacheExpand x(b);
+  return x.used ? x.bytes() : align256(g4::cache_part_bytes(cache_attn_params(b)));
 }
 
 static int cache_attn_expanded(const g4_cache_attn& p, CacheExpand& x, const void* q, g4_layout ql,
@@ -1054,17 +1065,24 @@ static int cache_attn_expanded(const g4_cache_attn& p, CacheExpand& x, const voi
   char* const fwd = ws + 2 * x.cu + 2 * x.operand;
   const int hkv = p.cache.num_kv_heads, d = p.cache.head_dim;
   const g4_layout lay{0, (int64_t)hkv * d, d};
-  g4::ExpandParams e{p.table, p.cu_seqlens_q, p.total_q, p.max_seqlen_q, p.max_seqlen_k,
-                     p.window, p.num_sinks, x.p.seqlen_k, cu_q, cu_k};
-  hipError_t err = g4::launch_cache_expand_lengths(e, st);
-  if (err != hipSuccess) return hip_fail(err, "cache attention lengths");
-  g4::GatherParams g{p.cache, p.table, cu_k, x.rows, {k, v}, {lay, lay}, cu_q, p.max_seqlen_k,
-                     p.window, p.num_sinks};
-  err = g4::launch_cache_gather(g, st);
-  if (err != hipSuccess) return hip_fail(err, "cache attention rows");
   x.p.cu_seqlens_q = cu_q;
   x.p.cu_seqlens_k = cu_k;
-  return fwd_impl(&x.p, q, ql, k, lay, v, lay, o, ol, lse, fwd, x.fwd, st, p.num_sinks);
+  for (int s0 = 0; s0 < p.table.batch; s0 += x.per) {
+    // (a last step of fewer sequences takes the workspace of a full one)
+    x.p.num_seqs = std::min(x.per, p.table.batch - s0);
+    const g4_page_table table{p.table.pages + (int64_t)s0 * p.table.width, p.table.seq_lens + s0,
+                              x.p.num_seqs, p.table.width};
+    g4::ExpandParams e{table, p.cu_seqlens_q + s0, p.total_q, p.max_seqlen_q, p.max_seqlen_k,
+                       p.window, p.num_sinks, x.p.seqlen_k, cu_q, cu_k};
+    hipError_t err = g4::launch_cache_expand_lengths(e, st);
+    if (err != hipSuccess) return hip_fail(err, "cache attention lengths");
+    g4::GatherParams g{p.cache, table, cu_k, (int64_t)x.p.num_seqs * x.p.seqlen_k, {k, v},
+                       {lay, lay}, cu_q, p.max_seqlen_k, p.window, p.num_sinks};
+    err = g4::launch_cache_gather(g, st);
+    if (err != hipSuccess) return hip_fail(err, "cache attention rows");
+    G4_TRY(fwd_impl(&x.p, q, ql, k, lay, v, lay, o, ol, lse, fwd, x.fwd, st, p.num_sinks));
+  }
+  return G4_OK;
 }
 
 int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void* o, g4_layout ol,
@@ -1075,8 +1093,9 @@ int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void*
   G4_TRY(check_operand(q, ql, "q"));
   G4_TRY(check_operand(o, ol, "o"));
   if (lse == nullptr) return fail(G4_ERR_INVALID, "lse is NULL");
-  g4::CacheAttnParams a = cache_attn_params(*p);
-  CacheExpand x(*p);
+  const g4_cache_attn b = cache_attn_bounded(*p);
+  g4::CacheAttnParams a = cache_attn_params(b);
+  CacheExpand x(b);
   const size_t need = x.used ? x.bytes() : align256(g4::cache_part_bytes(a));
   if (ws == nullptr || ws_bytes < need || ((uintptr_t)ws) % 256) {
     char buf[128];
@@ -1084,7 +1103,7 @@ int g4_cache_attn_fwd(const g4_cache_attn* p, const void* q, g4_layout ql, void*
     return fail(G4_ERR_WORKSPACE, "cache attention workspace: %s", buf);
   }
   if (x.used)
-    return cache_attn_expanded(*p, x, q, ql, o, ol, lse, (char*)ws, (hipStream_t)stream);
+    return cache_attn_expanded(b, x, q, ql, o, ol, lse, (char*)ws, (hipStream_t)stream);
   a.q = (const __bf16*)q;
   a.o = (__bf16*)o;
   a.lse = lse;

@@ -106,8 +106,8 @@ struct VisibleRows {
   }
 };
 
-// Cumulative lengths of the closed-up sequences and of the queries, both within
-// their buffers whatever the lengths on the device are.
+// Cumulative lengths of the closed-up sequences and (from cu_q[0] on) of the queries,
+// both within their buffers whatever the lengths on the device are.
 struct ExpandParams {
   g4_page_table tab;
   const int* cu_q;
@@ -130,9 +130,8 @@ struct CacheAttnParams {
   float* lse;
   g4_layout ql, ol;
   // Set by the launcher (g4_cache_attn.hip): workgroups at most, groups and queries of
-  // a set, sets of a sequence at most; the parts' heads, and partial rows of the
-  // segments that several parts share.
-  int parts, set_groups, set_queries, sets;
+  // a set; the parts' heads, and their sums of the segments that several parts share.
+  int parts, set_groups, set_queries;
   struct PartHead* heads;
   float* part;
 };

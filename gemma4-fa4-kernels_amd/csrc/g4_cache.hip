@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {
 __global__ void __launch_bounds__(256) expand_lengths_kernel(ExpandParams a) {
   __shared__ int64_t lds[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t base_q = 0, base_k = 0;
+  const int64_t first_q = min(max((int64_t)a.cu_q[0], (int64_t)0), a.total_q);
+  int64_t base_q = first_q, base_k = 0;
   for (int s0 = 0; s0 < a.tab.batch; s0 += 256) {
     const int s = s0 + tid;
     int64_t q = 0, k = 0;
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(256) expand_lengths_kernel(ExpandParams a) {
       a.out_k[s + 1] = (int)(before_k + k);
     }
   }
-  if (tid == 0) a.out_q[0] = a.out_k[0] = 0;
+  if (tid == 0) a.out_q[0] = (int)first_q, a.out_k[0] = 0;
 }
 
 hipError_t launch_cache_expand_lengths(const ExpandParams& a, hipStream_t stream) {

@@ -20,9 +20,9 @@
 // into equal parts, one workgroup each, so that the longest sequence of a batch
 // does not decide its time.  A group's waves take its tiles in turn and add up
 // through LDS; a segment inside one part is finished there, else the parts' sums go
-// to the workspace (slot = part + segment: along the parts both only grow, so no
-// two pairs share one), and the second launch has a workgroup for each cut: those
-// of one segment share its rows' elements evenly.
+// to the workspace (two slots a part: only the segments it begins and ends in can be
+// cut), and the second launch has a workgroup for each cut: those of one segment
+// share its rows' elements evenly.
 //
 // Bound by HBM for long batches (1 byte an element of K and V), by the chain of
 // launch, table, page and merge latencies for short ones.
@@ -199,13 +199,19 @@ __device__ __forceinline__ bool find_part(const CacheAttnParams& a, int part, in
 
 }  // namespace
 
-// What a part leaves for the merge: the segment it begins in (its number, first tile,
-// tiles, KV head, first query's row and rows) and the batch's tiles and parts.
+// What a part leaves for the merge: the segment it begins in (its first tile, tiles, KV
+// head, first query's row and rows) and the batch's tiles and parts.
 struct PartHead {
-  int64_t tiles, seg0, segment;
+  int64_t tiles, seg0;
   int parts, n, kvh, q_row, rows, pad;
 };
-static_assert(sizeof(PartHead) == 48, "a part's head");
+static_assert(sizeof(PartHead) == 40, "a part's head");
+
+// Slot of a part's sums for a segment that begins at tile seg0: the first slot for the
+// segment that the part begins in, the second for one that begins within it.
+__device__ __forceinline__ int64_t part_slot(int part, int64_t part_lo, int64_t seg0) {
+  return 2 * (int64_t)part + (seg0 > part_lo);
+}
 
 template <int D>
 struct CacheWave {
@@ -362,8 +368,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
   seg0 += (int64_t)kvh * range.n;
   const int grp = a.num_q_heads / hkv, gsh = __builtin_ctz(grp);
   if (tid == 0)
-    a.heads[part] = PartHead{f.tiles, seg0, ((int64_t)s * a.sets + set) * hkv + kvh, f.parts,
-                             range.n, kvh, sq.q0 + set * a.set_queries,
+    a.heads[part] = PartHead{f.tiles, seg0, f.parts, range.n, kvh,
+                             sq.q0 + set * a.set_queries,
                              min(a.set_queries, sq.lq - set * a.set_queries) << gsh, 0};
   const int blocks = a.c.page_size / kTile;
   while (true) {
@@ -460,8 +466,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
     barrier_lds();
     const bool whole = x0 == 0 && x1 == range.n;
     const int nrows = (set_last - set_first + 1) << gsh;
-    const int64_t segment = ((int64_t)s * a.sets + set) * hkv + kvh;
-    float* const part_o = a.part + (part + segment) * (int64_t)(sets * kGroupRows * (D + 2));
+    float* const part_o =
+        a.part + part_slot(part, f.lo, seg0) * (int64_t)(sets * kGroupRows * (D + 2));
     constexpr int kCols = D / 4;  // threads of a row, four elements each
     for (int r = tid / kCols; r < nrows; r += 256 / kCols) {
       const int d = tid % kCols * 4, g = r / kGroupRows, ri = r % kGroupRows;
@@ -532,7 +538,10 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
   const int grp = a.num_q_heads / a.c.num_kv_heads, gsh = __builtin_ctz(grp);
   const int set_rows = a.set_groups * kGroupRows;
   const int64_t slot = (int64_t)set_rows * (D + 2);
-  const float* const part = a.part + (w0 + hd.segment) * slot;
+  // the segment's parts: its first part's slot, then the first slots of the following
+  const float* const part0 = a.part + part_slot(w0, tiles * w0 / parts, hd.seg0) * slot;
+  const float* const part1 = a.part + 2 * (int64_t)(w0 + 1) * slot;
+  const auto sums = [&](int c) { return c == 0 ? part0 : part1 + 2 * (int64_t)(c - 1) * slot; };
 
   const int units = hd.rows * (D / 4);  // four elements of a row each
   const int u0 = (int)((int64_t)units * (w - w0 - 1) / (n - 1));
@@ -544,8 +553,7 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
     const int u = ub + tid / subs, sub = tid % subs;
     const bool mine = u < u1;
     const int r = mine ? u / (D / 4) : 0, d = u % (D / 4) * 4;
-    const float* const ml = part + set_rows * D + 2 * r;
-    const float* const po = part + r * D + d;
+    const int ml = set_rows * D + 2 * r, po = r * D + d;
     float mx = kNegInf, sum = 0.f;
     f32x4 acc = {};
     if (mine) {
@@ -556,8 +564,9 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const int c = min(c0 + v * subs, n - 1);
-          ml4[v] = *(const f32x2*)(ml + c * slot);
-          o4[v] = *(const f32x4*)(po + c * slot);
+          const float* const part = sums(c);
+          ml4[v] = *(const f32x2*)(part + ml);
+          o4[v] = *(const f32x4*)(part + po);
         }
         float m_new = mx;
 #pragma unroll
@@ -611,17 +620,12 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
 // Workgroups that are resident at once.
 static int cache_parts(int head_dim) { return head_dim == 256 ? 512 : 256; }
 
-static int64_t cache_segments(const CacheAttnParams& a) {
-  return (int64_t)a.tab.batch * a.sets * a.c.num_kv_heads;
-}
-
 // Groups of a set: as many as the batch's longest run of new tokens fills.
 static void cache_sets(CacheAttnParams* a) {
   const int grp = a->num_q_heads / a->c.num_kv_heads;
   const int64_t rows = (int64_t)a->max_q * grp;
   a->set_groups = rows <= kGroupRows ? 1 : rows <= 2 * kGroupRows ? 2 : 4;
   a->set_queries = a->set_groups * kGroupRows / grp;
-  a->sets = (a->max_q + a->set_queries - 1) / a->set_queries;
   a->parts = cache_parts(a->c.head_dim);
 }
 
@@ -631,8 +635,7 @@ static size_t heads_bytes(const CacheAttnParams& a) {
 
 size_t cache_part_bytes(CacheAttnParams a) {
   cache_sets(&a);
-  const int64_t slots = a.parts + cache_segments(a);
-  return heads_bytes(a) + (size_t)slots * a.set_groups * kGroupRows * (a.c.head_dim + 2) * 4;
+  return heads_bytes(a) + (size_t)2 * a.parts * a.set_groups * kGroupRows * (a.c.head_dim + 2) * 4;
 }
 
 template <int D>

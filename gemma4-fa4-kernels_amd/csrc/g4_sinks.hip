@@ -41,13 +41,14 @@ __device__ __forceinline__ int sink_chunks(const SinkParams& a, int s) {
   return q.lk > a.b.p.window && q.lq > 0 ? (q.lq + a.chunk - 1) / a.chunk : 0;
 }
 
-// Sequence and chunk of slot x (slots number the chunks of all sequences);
-// false past the last.  Every lane of the wave calls it.
-__device__ __forceinline__ bool sink_slot(const SinkParams& a, int x, int& s, int& c) {
+// Sequence s of item x where sequence j has count(j) items, x's number c among them and
+// the items before them; false past the last.  Every lane of the wave calls it.
+template <class Count>
+__device__ __forceinline__ bool sink_item(const SinkParams& a, int x, Count count, int& s, int& c) {
   const int lane = __lane_id();
   int base = 0;
   for (int s0 = 0; s0 < a.b.p.num_seqs; s0 += 64) {
-    const int n = s0 + lane < a.b.p.num_seqs ? sink_chunks(a, s0 + lane) : 0;
+    const int n = s0 + lane < a.b.p.num_seqs ? count(s0 + lane) : 0;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -66,7 +67,7 @@ __device__ __forceinline__ bool sink_slot(const SinkParams& a, int x, int& s, in
   return false;
 }
 
-// Slots before sequence s.
+// Slots (the chunks of all sequences in order) before sequence s.
 __device__ __forceinline__ int sink_slots_before(const SinkParams& a, int s) {
   int n = 0;
   for (int j = __lane_id(); j < s; j += 64) n += sink_chunks(a, j);
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % p.num_kv_heads, slot = blockIdx.x / p.num_kv_heads;
   int s, chunk;
-  if (!sink_slot(sp, slot, s, chunk)) return;
+  if (!sink_item(sp, slot, [&](int j) { return sink_chunks(sp, j); }, s, chunk)) return;
   const Seq sq = resolve_seq(p, s);
   const int off = sq.lk - sq.lq;
   const int grp = p.num_q_heads / p.num_kv_heads;
@@ -221,11 +222,15 @@ __global__ void __launch_bounds__(256, 1) sinks_bwd_kernel(SinkParams sp) {
 __global__ void __launch_bounds__(64) sinks_sum_kernel(SinkParams sp) {
   const BwdParams& a = sp.b;
   const g4_problem& p = a.p;
-  const int kvh = blockIdx.x % p.num_kv_heads, s = blockIdx.x / p.num_kv_heads;
+  const int kvh = blockIdx.x % p.num_kv_heads;
   const int r = blockIdx.y % a.sinks, which = blockIdx.y / a.sinks;
+  int s, c0;  // of the sequences longer than the window
+  if (!sink_item(sp, blockIdx.x / p.num_kv_heads, [&](int j) { return sink_chunks(sp, j) > 0; }, s,
+                 c0))
+    return;
   const int n = sink_chunks(sp, s);
   const Seq sq = resolve_seq(p, s);
-  if (n == 0 || r >= sq.lk) return;
+  if (r >= sq.lk) return;
   const int first = sink_slots_before(sp, s);
   const int lane = threadIdx.x;
   const int64_t pitch = (int64_t)p.num_kv_heads * 2 * kSinkKeys * D;
@@ -245,10 +250,14 @@ static int sink_chunk(const g4_problem& p) {
   return (int)((rows / 512 + 31) / 32 * 32) + (rows < 512 ? 32 : 0);
 }
 
-// Chunks at most: sequences that a window does not cover have more keys than it.
+// Sequences that the window does not cover at most (they have more keys than it), and
+// their chunks.
+static int64_t sink_sequences(const g4_problem& p) {
+  return std::min<int64_t>(p.num_seqs, k_stream_tokens(p) / ((int64_t)p.window + 1));
+}
 static int64_t sink_slots(const g4_problem& p) {
-  const int64_t longer = std::min<int64_t>(p.num_seqs, k_stream_tokens(p) / (p.window + 1));
-  return q_stream_tokens(p) / sink_chunk(p) + longer;
+  const int64_t longer = sink_sequences(p);
+  return longer ? q_stream_tokens(p) / sink_chunk(p) + longer : 0;
 }
 
 size_t sinks_part_bytes(const g4_problem& p) {
@@ -273,7 +282,7 @@ hipError_t launch_sinks_bwd(const BwdParams& b, float* part, hipStream_t stream)
   hipLaunchKernelGGL(sinks_bwd_kernel, dim3((unsigned)blocks), dim3(256), kLdsBytes, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sinks_sum_kernel, dim3((unsigned)(b.p.num_seqs * b.p.num_kv_heads),
+  hipLaunchKernelGGL(sinks_sum_kernel, dim3((unsigned)(sink_sequences(b.p) * b.p.num_kv_heads),
                                             (unsigned)(2 * b.sinks)),
                      dim3(64), 0, stream, a);
   return hipGetLastError();

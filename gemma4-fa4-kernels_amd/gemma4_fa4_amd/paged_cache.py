@@ -222,7 +222,8 @@ def paged_cache_attention(
 
     A few new tokens per sequence are computed from the pages as they lie; from more
     than 128 query rows per KV head on (192 at head dim 256), what the batch can see is laid out as bf16 rows
-    in a workspace (``4 * batch * tokens * Hkv * head_dim`` bytes, up to 8 GiB).
+    in a workspace (``4 * tokens * Hkv * head_dim`` bytes a sequence, as many sequences
+    at a time as fit 8 GiB).
     """
     if q.ndim != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be a rank-3 BF16 (T, H, D) tensor")

@@ -230,6 +230,44 @@ def test_a_table_narrower_than_the_lengths():
     assert torch.isfinite(out[0]).all() and out[1].isnan().all()
 
 
+def test_a_cache_past_4_gib():
+    # offsets past 32 bits: the sequences lie in a cache's last pages
+    pages, hkv, page, d = 41000, 4, 64, 512
+    cache = empty_cache(pages, hkv, page, d)
+    assert cache.k.numel() > 5 << 30
+    lens, new = [200, 70], [1, 1]
+    table = [[pages - 1, pages - 7, pages - 2, 5], [pages - 3, 33000, -1, -1]]
+    k, v = (queries(60 + i, 270, hkv, d, 20.0) for i in range(2))
+    g4.paged_cache_append(cache, k, v, ints(table), ints(lens), ints(cu_of(lens)))
+    q = queries(62, 2, 32, d)
+    out, lse = attend(q, cache, table, lens, new)
+    check_attention(q, cache, table, lens, new, out, lse)
+    got, _ = g4.paged_cache_gather(cache, ints(table), ints(lens), ints(cu_of(lens)), 270)
+    assert (got.float() - k.float()).abs().max() <= 2.0 ** -4 * k.float().abs().max()
+    g4.copy_pages(cache, ints([pages - 1, 33000]), ints([40000, 0]))
+    table[0][0], table[1][1] = 40000, 0
+    again = attend(q, cache, table, lens, new)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("bound", [1, 300])
+def test_a_batch_without_queries(bound):
+    cache, table = filled_cache(21, [50, 60], 2, 32, 256)
+    q = queries(21, 4, 16, 256)
+    out, lse = g4.paged_cache_attention(q, cache, ints(table), ints([50, 60]), ints([0, 0, 0]),
+                                        max_seqlen_q=bound, max_seqlen_k=60)
+    assert out.isnan().all() and lse.isnan().all()  # (the fixture's fill: nothing is written)
+
+
+def test_chunks_of_more_sequences_than_fit_at_once():
+    # a generous bound of the lengths: 8 GiB hold the rows of 3 sequences of 700000 tokens
+    lens, new = [300, 40, 180, 260, 90, 150, 70], [50, 40, 33, 1, 0, 60, 35]
+    cache, table = filled_cache(22, lens, 4, 64, 256)
+    q = queries(22, sum(new), 32, 256)
+    out, lse = attend(q, cache, table, lens, new, max_k=700000)
+    check_attention(q, cache, table, lens, new, out, lse)
+
+
 def test_strided_queries_and_another_stream():
     lens, new = [400, 77], [1, 3]
     cache, table = filled_cache(14, lens, 2, 64, 256)

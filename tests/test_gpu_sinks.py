@@ -110,6 +110,38 @@ def test_against_fp64(hkv, grp, window, sinks, lq, lk, ds_budget):
     check_gradients(grads, [t.cpu() for t in (dq, dk, dv)], [t.cpu() for t in base])
 
 
+def test_many_sequences_of_which_few_are_longer_than_the_window():
+    lk = [20, 90, 5, 64, 65, 30, 200] * 20 + [64] * 30
+    q, k, v, do, dlse = (t.to(DEV) for t in qkv(77, sum(lk), sum(lk), 4, 2, 256))
+    o, lse, *grads = stages(q, k, v, lk, lk, 64, 5, do, dlse)
+    c = cu(lk).tolist()
+    *_, dq, dk, dv = pc.sinks_fwd_bwd(q, k, v, c, c, 64, 5, do, dlse)
+    base = baseline(q, k, v, c, c, 64, 5, do, dlse)
+    check_gradients(grads, [t.cpu() for t in (dq, dk, dv)], [t.cpu() for t in base])
+
+
+@pytest.mark.parametrize("lq,lk", [(300, 300), (50, 400)])
+def test_the_library_takes_fixed_layouts(lq, lk):
+    # (B, S, H, D) with strides, bitwise as the packed call on the same rows
+    from gemma4_fa4_amd import ops
+
+    b, hkv, grp, window, sinks = 3, 2, 2, 64, 6
+    q, k, v, do, dlse = (t.to(DEV) for t in qkv(9, b * lq, b * lk, hkv * grp, hkv, 256))
+    want = stages(q, k, v, [lq] * b, [lk] * b, window, sinks, do, dlse)
+    plan = ops.make_plan(num_seqs=b, seqlen_q=lq, seqlen_k=lk, num_q_heads=hkv * grp,
+                         num_kv_heads=hkv, head_dim=256, window=window)
+    plan.num_sinks = sinks
+    q4, k4, v4, do4 = (t.view(b, -1, t.shape[1], 256) for t in (q, k, v, do))
+    k4 = torch.cat((k4, k4), 2)[:, :, :hkv]  # strided
+    o, lse = plan.forward(q4, k4, v4)
+    dlse4 = dlse.view(hkv * grp, b, lq).transpose(0, 1).contiguous()
+    grads = plan.backward(q4, k4, v4, o, do4, lse, dlse4)
+    assert torch.equal(o.flatten(0, 1), want[0])
+    assert torch.equal(lse.transpose(0, 1).reshape(hkv * grp, -1), want[1])
+    for x, y in zip(grads, want[2:]):
+        assert torch.equal(x.flatten(0, 1), y)
+
+
 def adapter(q, k, v, lq, lk, sinks):
     return g4.fa4_local_sinks_varlen_forward(
         q, k, v, cu(lq).to(DEV), cu(lk).to(DEV), max_seqlen_q=max(lq), max_seqlen_k=max(lk),
