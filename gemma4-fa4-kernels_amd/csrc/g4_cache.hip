@@ -11,8 +11,10 @@ namespace g4 {
 // rows.  Scales are powers of two: an e4m3 value divided by one keeps its bits
 // but where it falls below the type's normal range, so a growing scale costs a
 // block's earlier tokens next to nothing, and what a block holds does not
-// depend on how its tokens were dealt to the calls but there.  Memory-bound: a
-// row is read once (2 bytes an element) and written once (1 byte).
+// depend on how its tokens were dealt to the calls but there.  Bound by HBM: a
+// row is read once (2 bytes an element) and written once (1 byte): 19500 tokens of 16
+// heads of 256 in 99 us, 4.8 TB/s (with the heads' rows apart in the grid 109).  One
+// token a sequence is a chain of latencies: 64 sequences 6.7 us.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
@@ -117,7 +119,8 @@ hipError_t launch_cache_append(const AppendParams& a, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------
-// Gather.  One workgroup per (32 output rows of a sequence, head, K or V).
+// Gather.  One workgroup per (32 output rows of a sequence, head, K or V).  Bound by
+// HBM: 12500 tokens of 4 heads of 512 (51 MB read, 102 written) in 28 us, 5.5 TB/s.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {

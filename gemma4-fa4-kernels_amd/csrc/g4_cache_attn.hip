@@ -24,8 +24,12 @@
 // cut), and the second launch has a workgroup for each cut: those of one segment
 // share its rows' elements evenly.
 //
-// Bound by HBM for long batches (1 byte an element of K and V), by the chain of
-// launch, table, page and merge latencies for short ones.
+// Bound by HBM for long batches (1 byte an element of K and V: 2 x 100000 tokens of 4
+// heads of 512 in 145 us, 5.4 TB/s; 16 of 4096 to 8192 tokens 89 + 6 us, of which about
+// 8 are the way to the first tile), by the chain of launch, lengths, table, page and
+// merge for short ones (one window of 1024 tokens, 16 heads of 256: 11.6 + 5.4 us).
+// With one workgroup per (segment, row) the merge took 14 and 23 us (8 sequences of 5
+// new tokens) in place of 6 and 4.4.
 #include "g4_cache.h"
 
 namespace g4 {

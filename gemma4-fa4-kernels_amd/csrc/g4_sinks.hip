@@ -13,8 +13,13 @@
 // take 32 rows of one query head at a time: S = Q K^T and dP = dO V^T with keys
 // along lanes feed dV^T += dO^T P and dK^T += Q^T dS from registers.  The chunk's
 // dK and dV go to the workspace and a second launch adds the chunks in order (no
-// atomics).  Bound by HBM: Q and dO are read once more, 2 x 512 bytes a row, and
-// 64 bytes of dS written.
+// atomics).  Q and dO are read once more, 2 x 512 bytes a row, and 64 bytes of dS
+// written: bound by HBM, which one tile a wave in flight and one workgroup a CU (128 KB
+// of tiles, 256 accumulator registers) keep at 3.5 TB/s (32768 tokens 310 us; the next
+// tile held in registers spilled there, 349).  Adding dQ to the stored rows here instead
+// cost 4 x 512 bytes a row (558 us) and rounded it twice.
+#include <algorithm>
+
 #include "g4_kernels.h"
 
 namespace g4 {
@@ -244,10 +249,13 @@ __global__ void __launch_bounds__(64) sinks_sum_kernel(SinkParams sp) {
              4 * lane) = bf16x4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
 }
 
-// Queries of a chunk: about two workgroups per CU in all.
+// Queries of a chunk: one workgroup per CU for one sequence, about two for several,
+// whose last chunks are short (whole training calls, us, 256 / 512 workgroups: 2500
+// tokens 399 / 409, 5000 832 / 845, 20 sequences of 30000 tokens 3830 / 3780).
 static int sink_chunk(const g4_problem& p) {
   const int64_t rows = q_stream_tokens(p) * p.num_kv_heads;
-  return (int)((rows / 512 + 31) / 32 * 32) + (rows < 512 ? 32 : 0);
+  const int64_t chunk = (rows / (p.num_seqs == 1 ? 256 : 512) + 31) / 32 * 32;
+  return (int)std::max<int64_t>(chunk, 32);
 }
 
 // Sequences that the window does not cover at most (they have more keys than it), and
