@@ -1041,9 +1041,11 @@ struct CacheExpand {
   size_t bytes() const { return 2 * cu + 2 * operand + fwd; }
 };
 
-// A call's problem with its bounds no larger than its rows make them.
+// A call's problem with its bounds no larger than its rows make them.  (A window past
+// the longest sequence excludes nothing; position - window then stays an int.)
 static g4_cache_attn cache_attn_bounded(const g4_cache_attn& p) {
   g4_cache_attn b = p;
+  b.window = std::min(p.window, p.max_seqlen_k);
   b.max_seqlen_q = (int32_t)std::min<int64_t>(p.max_seqlen_q, std::max<int64_t>(p.total_q, 1));
   return b;
 }

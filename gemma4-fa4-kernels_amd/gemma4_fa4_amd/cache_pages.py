@@ -28,9 +28,9 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _require_gfx950
+from .attention import _is_python_int, _require_gfx950
 from .errors import UnsupportedMI355XPath
-from .paged_cache import PAGE_SIZES, PagedKVCache, _ints, _table
+from .paged_cache import _INT32_MAX, PAGE_SIZES, PagedKVCache, _ints, _table, _window
 
 
 def _pool(page_table, seq_lens, ref_counts, rows=None, name: str = ""):
@@ -39,6 +39,8 @@ def _pool(page_table, seq_lens, ref_counts, rows=None, name: str = ""):
     table = _table(page_table, seq_lens, device)
     if ref_counts.ndim != 1 or ref_counts.shape[0] < 1:
         raise ValueError("ref_counts must be a rank-1 (num_pages,) tensor")
+    if ref_counts.shape[0] > _INT32_MAX:
+        raise UnsupportedMI355XPath("ref_counts must have fewer than 2^31 pages")
     _ints(ref_counts, (ref_counts.shape[0],), device, "ref_counts")
     if rows is not None:
         _ints(rows, (table.batch,), device, name)
@@ -108,15 +110,16 @@ def release_pages(page_table, seq_lens, ref_counts, keep_lens, *, page_size: int
     """
     table, device = _pool(page_table, seq_lens, ref_counts, keep_lens, "keep_lens")
     _page_size(page_size)
-    if sliding_window is not None and sliding_window < 1:
-        raise ValueError("sliding_window must be positive")
+    window = _window(sliding_window)
+    if not _is_python_int(num_sinks):
+        raise TypeError("num_sinks must be a Python integer")
     if num_sinks < 0:
         raise ValueError("num_sinks must be >= 0")
     _require_gfx950(device)
     with _lib.device_scope(device):
         _lib.check(_lib.load().g4_pages_release(
             ctypes.byref(table), ref_counts.data_ptr(), ref_counts.shape[0], page_size,
-            keep_lens.data_ptr(), sliding_window or 0, num_sinks, _lib.raw_stream(device)))
+            keep_lens.data_ptr(), window, min(num_sinks, _INT32_MAX), _lib.raw_stream(device)))
 
 
 def compact_pages(page_table, ref_counts):
@@ -145,11 +148,14 @@ def copy_pages(cache: PagedKVCache, src: torch.Tensor, dst: torch.Tensor) -> Non
     Pairs with an entry that is no page (-1) are skipped.  A page may not be a
     destination twice, nor a source and a destination.
     """
+    desc = cache.descriptor()
     if src.ndim != 1:
         raise ValueError("src must be a rank-1 tensor")
+    if src.shape[0] > _INT32_MAX:
+        raise UnsupportedMI355XPath("one call copies fewer than 2^31 pages")
     for name, t in (("src", src), ("dst", dst)):
         _ints(t, (src.shape[0],), cache.device, name)
     with _lib.device_scope(cache.device):
         _lib.check(_lib.load().g4_pages_copy(
-            ctypes.byref(cache._desc), src.data_ptr(), dst.data_ptr(), src.shape[0],
+            ctypes.byref(desc), src.data_ptr(), dst.data_ptr(), src.shape[0],
             _lib.raw_stream(cache.device)))

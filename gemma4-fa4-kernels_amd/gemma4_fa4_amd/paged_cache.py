@@ -40,6 +40,7 @@ from .errors import UnsupportedMI355XPath
 CACHE_BLOCK = 32  # tokens that share a scale
 PAGE_SIZES = (32, 64, 128, 256)
 _E4M3 = torch.float8_e4m3fn
+_INT32_MAX = 2**31 - 1
 
 
 class PagedKVCache:
@@ -54,6 +55,25 @@ class PagedKVCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
                  v_scale: torch.Tensor):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._pointers = None
+        self.descriptor()
+
+    def descriptor(self) -> G4PagedCache:
+        """The tensors as the library takes them, checked anew where their memory changed."""
+        pointers = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                    self.v_scale.data_ptr())
+        if pointers != self._pointers:
+            self._check()
+            self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = self.k.shape
+            self.device = self.k.device
+            self._desc = G4PagedCache(*pointers, self.num_pages, self.num_kv_heads,
+                                      self.head_dim, self.page_size)
+            self._pointers = pointers
+        return self._desc
+
+    def _check(self) -> None:
+        k, v = self.k, self.v
         for name, t in (("k", k), ("v", v)):
             if t.ndim != 4 or t.dtype != _E4M3:
                 raise ValueError(f"cache {name} must be a rank-4 float8_e4m3fn tensor "
@@ -66,25 +86,20 @@ class PagedKVCache:
         if page_size not in PAGE_SIZES or head_dim not in (256, 512):
             raise UnsupportedMI355XPath(
                 "the paged cache covers page sizes 32, 64, 128 and 256 and head dims 256 and 512")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        for name, t in (("k_scale", self.k_scale), ("v_scale", self.v_scale)):
             if t.dtype != torch.float32 or t.shape != (pages, heads, page_size // CACHE_BLOCK):
                 raise ValueError(f"cache {name} must be a float32 tensor "
                                  "(num_pages, num_kv_heads, page_size // 32)")
-        tensors = (k, v, k_scale, v_scale)
+        tensors = (k, v, self.k_scale, self.v_scale)
         if any(t.device != k.device for t in tensors):
             raise ValueError("the cache's tensors must share a device")
         if not all(t.is_contiguous() for t in tensors):
             raise ValueError("the cache's tensors must be contiguous")
-        if len({t.untyped_storage().data_ptr() for t in (k, v)}) != 2:
-            raise ValueError("cache k and v must be distinct tensors")
         _check_real_operands((k, v), ("k", "v"), label="cache k and v")
+        ends = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in tensors)
+        if any(start < end for (_, end), (start, _) in zip(ends, ends[1:])):
+            raise ValueError("the cache's tensors must be distinct, without memory in common")
         _require_gfx950(k.device)
-        self.k, self.v, self.k_scale, self.v_scale = tensors
-        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
-        self.device = k.device
-        self._desc = G4PagedCache(
-            k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            pages, heads, head_dim, page_size)
 
     @classmethod
     def empty(cls, num_pages: int, *, num_kv_heads: int, head_dim: int, page_size: int = 64,
@@ -108,12 +123,25 @@ def _ints(t: torch.Tensor, shape, device, name: str) -> None:
 def _table(page_table: torch.Tensor, seq_lens: torch.Tensor | None, device) -> G4PageTable:
     if page_table.ndim != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
         raise ValueError("page_table must be a rank-2 (batch, width) tensor")
+    if page_table.numel() > _INT32_MAX:
+        raise UnsupportedMI355XPath("page_table must have fewer than 2^31 entries")
     batch, width = page_table.shape
     _ints(page_table, (batch, width), device, "page_table")
     if seq_lens is None:
         return G4PageTable(page_table.data_ptr(), page_table.data_ptr(), batch, width)
     _ints(seq_lens, (batch,), device, "seq_lens")
     return G4PageTable(page_table.data_ptr(), seq_lens.data_ptr(), batch, width)
+
+
+def _window(sliding_window: int | None) -> int:
+    """The library's window: 0 for none, and no more than its int holds (which is all)."""
+    if sliding_window is None:
+        return 0
+    if not _is_python_int(sliding_window):
+        raise TypeError("sliding_window must be a Python integer")
+    if sliding_window < 1:
+        raise ValueError("sliding_window must be positive")
+    return min(sliding_window, _INT32_MAX)
 
 
 def _no_autograd(*tensors) -> None:
@@ -140,6 +168,7 @@ def paged_cache_append(
     without a page are dropped, rows past ``cu_seqlens[-1]`` are not read.  A page
     may receive tokens of one sequence only (``reserve_pages`` sees to that).
     """
+    desc = cache.descriptor()
     if k.ndim != 3 or v.ndim != 3 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("k and v must be rank-3 BF16 (T, H, D) tensors")
     if k.shape[1:] != (cache.num_kv_heads, cache.head_dim) or v.shape != k.shape:
@@ -156,7 +185,7 @@ def paged_cache_append(
     _check_real_operands((k, v), ("k", "v"), label="k and v")
     with _lib.device_scope(cache.device):
         _lib.check(_lib.load().g4_cache_append(
-            ctypes.byref(cache._desc), ctypes.byref(table), cu_seqlens.data_ptr(), k.shape[0],
+            ctypes.byref(desc), ctypes.byref(table), cu_seqlens.data_ptr(), k.shape[0],
             k.data_ptr(), G4Layout(0, k.stride(0), k.stride(1)),
             v.data_ptr(), G4Layout(0, v.stride(0), v.stride(1)),
             _lib.raw_stream(cache.device)))
@@ -175,6 +204,7 @@ def paged_cache_gather(
     stands for); rows of tokens past ``seq_lens[b]`` or without a page are zero.
     Rows past ``cu_seqlens[-1]`` are not written.
     """
+    desc = cache.descriptor()
     if type(total) is not int or total < 0:
         raise ValueError("total must be a non-negative Python integer")
     table = _table(page_table, seq_lens, cache.device)
@@ -186,7 +216,7 @@ def paged_cache_gather(
         layout = G4Layout(0, k.stride(0), k.stride(1))
         with _lib.device_scope(cache.device):
             _lib.check(_lib.load().g4_cache_gather(
-                ctypes.byref(cache._desc), ctypes.byref(table), cu_seqlens.data_ptr(), total,
+                ctypes.byref(desc), ctypes.byref(table), cu_seqlens.data_ptr(), total,
                 k.data_ptr(), layout, v.data_ptr(), layout, _lib.raw_stream(cache.device)))
     return k, v
 
@@ -221,10 +251,11 @@ def paged_cache_attention(
     window nor sinks; query heads are 1, 2, 4 or 8 times the cache's.
 
     A few new tokens per sequence are computed from the pages as they lie; from more
-    than 128 query rows per KV head on (192 at head dim 256), what the batch can see is laid out as bf16 rows
-    in a workspace (``4 * tokens * Hkv * head_dim`` bytes a sequence, as many sequences
-    at a time as fit 8 GiB).
+    than 128 query rows per KV head on (192 at head dim 256), what the batch can see is
+    laid out as bf16 rows in a workspace (``4 * tokens * Hkv * head_dim`` bytes a
+    sequence, as many sequences at a time as fit 8 GiB).
     """
+    desc = cache.descriptor()
     if q.ndim != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be a rank-3 BF16 (T, H, D) tensor")
     total, heads, head_dim = q.shape
@@ -240,8 +271,9 @@ def paged_cache_attention(
         raise TypeError("max_seqlen_q and max_seqlen_k must be Python integers")
     if not (1 <= max_seqlen_q <= _MAX_LENGTH and 1 <= max_seqlen_k <= _MAX_LENGTH):
         raise ValueError("max_seqlen_q and max_seqlen_k must be in [1, 2^30]")
-    if sliding_window is not None and sliding_window < 1:
-        raise ValueError("sliding_window must be positive")
+    window = _window(sliding_window)
+    if not _is_python_int(num_sinks):
+        raise TypeError("num_sinks must be a Python integer")
     if not 0 <= num_sinks <= _MAX_SINKS:
         raise UnsupportedMI355XPath(f"num_sinks must be in [0, {_MAX_SINKS}]")
     if sliding_window is None and num_sinks:
@@ -258,8 +290,8 @@ def paged_cache_attention(
     _validate_layout(q, name="q")
     _check_real_operands((q,), ("q",), label="q")
     lib = _lib.load()
-    prob = G4CacheAttn(cache._desc, table, cu_seqlens_q.data_ptr(), total, heads,
-                       max_seqlen_q, max_seqlen_k, sliding_window or 0, num_sinks)
+    prob = G4CacheAttn(desc, table, cu_seqlens_q.data_ptr(), total, heads,
+                       max_seqlen_q, max_seqlen_k, window, num_sinks)
     ref = ctypes.byref(prob)
     ws = torch.empty(lib.g4_cache_attn_workspace_bytes(ref), dtype=torch.uint8, device=q.device)
     with _lib.device_scope(q.device):

@@ -333,3 +333,17 @@ def test_a_captured_decode_loop():
         assert (state[0][0][0, 1].item() >= 0) == (i < 40)
     assert state[0][1].tolist() == [n + 44 for n in lens]
     assert (state[0][0][0] >= 0).tolist() == [True, False, True, True, False, False]
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**32 + 1, 400])
+def test_a_window_past_every_length(window):
+    """As no window, also for more new tokens than the sequence has."""
+    for lens, new in (([300, 5, 60], [2, 9, 60]), ([300, 5, 60], [120, 100, 60])):
+        cache, table = filled_cache(30, lens, 2, 64, 256)
+        q = queries(30, sum(new), 8, 256)
+        want = attend(q, cache, table, lens, new)
+        got = attend(q, cache, table, lens, new, window=window)
+        check_attention(q, cache, table, lens, new, *got)
+        got = attend(q, cache, table, lens, new, window=window, sinks=3)
+        check_attention(q, cache, table, lens, new, *got)
+        assert torch.equal(torch.isneginf(got[1]), torch.isneginf(want[1]))

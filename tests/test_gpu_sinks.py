@@ -258,3 +258,30 @@ def test_a_captured_single_token_step():
         want = plan.forward(q, k, v)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     check_forward(q, k, v, [1, 1], lk, 1024, 4, *got, heads=[0, 31])
+
+
+@pytest.mark.parametrize("ds_budget", [0, -1])
+def test_a_captured_backward(ds_budget):
+    from gemma4_fa4_amd import ops
+
+    n = [200, 90]
+    q, k, v, do, dlse = (t.to(DEV) for t in qkv(12, 290, 290, 4, 2, 256))
+    plan = ops.make_plan(num_seqs=2, seqlen_q=200, seqlen_k=200, num_q_heads=4, num_kv_heads=2,
+                         head_dim=256, window=64, cu_q=cu(n).to(DEV), cu_k=cu(n).to(DEV),
+                         total_q=290, total_k=290, ds_budget=ds_budget)
+    plan.num_sinks = 4
+
+    def step():
+        o, lse = plan.forward(q, k, v)
+        return (o, lse, *plan.backward(q, k, v, o, do, lse, dlse))
+
+    step()  # (launch attributes are set outside the capture)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        q.copy_(qkv(60 + i, 290, 1, 4, 2, 256)[0])
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check_forward(q, k, v, n, n, 64, 4, *got[:2])

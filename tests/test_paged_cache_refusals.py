@@ -276,3 +276,60 @@ def test_the_library_refuses_attention():
     assert call(nbytes=255) == _lib.G4_ERR_WORKSPACE
     assert call(ws=t + 16) == _lib.G4_ERR_WORKSPACE
     assert call(rows=0, q=None, lse=None) == _lib.G4_OK
+
+
+def test_a_cache_whose_tensors_share_memory(monkeypatch):
+    monkeypatch.setattr(pcm, "_require_gfx950", lambda device: None)
+    k, v, ks, vs = tensors()
+    with pytest.raises(ValueError, match="memory in common"):
+        g4.PagedKVCache(k, v, ks, ks)
+    pool = torch.zeros(7, 2, 64, 256, dtype=torch.uint8).view(E4M3)
+    with pytest.raises(ValueError, match="memory in common"):
+        g4.PagedKVCache(pool[:4], pool[3:], ks, vs)
+    pool = torch.zeros(2, 4, 2, 64, 256, dtype=torch.uint8).view(E4M3)
+    assert g4.PagedKVCache(pool[0], pool[1], ks, vs).num_pages == 4  # two parts of one tensor
+
+
+def test_a_cache_whose_memory_changes(cache):
+    old = cache.descriptor()
+    assert cache.descriptor() is old
+    cache.k, cache.v, cache.k_scale, cache.v_scale = tensors(pages=9, d=512)
+    assert cache.descriptor().num_pages == 9 and cache.descriptor().k == cache.k.data_ptr()
+    cache.v = tensors()[1]
+    with pytest.raises(ValueError, match="same shape"):
+        g4.paged_cache_append(cache, **append_args())
+    with pytest.raises(ValueError, match="same shape"):
+        g4.copy_pages(cache, *torch.zeros(2, 3, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("window", [64.0, True, torch.tensor(64)])
+def test_windows_and_sinks_are_integers(cache, window):
+    args = attention_args()
+    with pytest.raises(TypeError, match="sliding_window"):
+        g4.paged_cache_attention(args["q"], cache, **{k: v for k, v in args.items() if k != "q"},
+                                 sliding_window=window)
+    with pytest.raises(TypeError, match="num_sinks"):
+        g4.paged_cache_attention(args["q"], cache, **{k: v for k, v in args.items() if k != "q"},
+                                 sliding_window=64, num_sinks=window)
+    pool = pool_args() | dict(keep_lens=torch.zeros(3, dtype=torch.int32), page_size=64)
+    with pytest.raises(TypeError, match="sliding_window"):
+        g4.release_pages(**pool, sliding_window=window)
+    with pytest.raises(TypeError, match="num_sinks"):
+        g4.release_pages(**pool, sliding_window=64, num_sinks=window)
+
+
+def test_a_window_past_32_bits_is_not_cut_to_its_low_ones():
+    assert pcm._window(2**32 + 1) == pcm._window(2**31 - 1) == 2**31 - 1
+    assert pcm._window(None) == 0 and pcm._window(5) == 5
+
+
+def test_tables_pools_and_lists_past_32_bits():
+    i = dict(dtype=torch.int32, device="meta")
+    pool = dict(page_table=torch.zeros(3, 4, **i), seq_lens=torch.zeros(3, **i),
+                ref_counts=torch.zeros(6, **i))
+    with pytest.raises(g4.UnsupportedMI355XPath, match="2\\^31"):
+        pcm._table(torch.zeros(2**16, 2**15, **i), None, torch.device("meta"))
+    from gemma4_fa4_amd import cache_pages
+
+    with pytest.raises(g4.UnsupportedMI355XPath, match="2\\^31"):
+        cache_pages._pool(pool["page_table"], None, torch.zeros(2**31, **i))
