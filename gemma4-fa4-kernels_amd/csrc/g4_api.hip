@@ -995,16 +995,21 @@ static g4::CacheAttnParams cache_attn_params(const g4_cache_attn& p) {
 
 // Larger chunks of new tokens: the visible rows of every sequence as bf16 in the
 // workspace, and the forward of g4_attn_fwd over them.  Reading pages as they lie
-// costs the cache once per 64 query rows of a KV head and a conversion per 16, the
-// copy five times the cache's bytes once, whatever the rows.  As they lie / laid out,
-// us, head dim 512 (8 heads a KV head), by rows: 16 x 8192 tokens 64: 269 / 634, 128:
-// 505 / 644, 192: 756 / 750; 16 x 1000 64: 65 / 87, 128: 130 / 96; 1 x 8192 128: 63 /
-// 86, 256: 83 / 86.  Head dim 256 with a window of 1024: 16 x 8192 128: 112 / 204, 192:
-// 192 / 218; 16 x 1000 192: 183 / 190; 1 x 1000 192: 43 / 50.
+// costs the cache once per 64 query rows of a KV head and a conversion per 64 (head dim
+// 512) or 16, the copy five times the cache's bytes once, whatever the rows, and three
+// launches more.  As they lie / laid out, us, by rows of a KV head: head dim 512, 1 x
+// 8192 tokens 192: 58 / 85, 320: 74 / 88, 448: 87 / 91; 16 x 8192 192: 283 / 607, 448:
+// 568 / 838; 16 x 1000 320: 99 / 106, 448: 122 / 107; 1 x 12000 512: 122 / 114.  Head
+// dim 256 with a window of 1024: 1 x 8192 256: 37 / 54, 320: 48 / 55, 2 x 8192 256: 53 /
+// 58, 320: 60 / 59, 4 x 8192 200: 67 / 65, 256: 76 / 67, 16 x 8192 200: 163 / 178, 256:
+// 183 / 185, 16 x 700 256: 125 / 107.
 // Sequences are taken as many at a time as fit kMost bytes, at least one.
 struct CacheExpand {
   // query rows of a KV head that are read as they lie
-  static int as_they_lie(int head_dim) { return head_dim == 512 ? 128 : 192; }
+  static int64_t as_they_lie(const g4_cache_attn& a) {
+    if (a.cache.head_dim == 512) return 448;
+    return a.table.batch <= 2 ? 320 : 192;
+  }
   static constexpr int64_t kMost = int64_t(8) << 30;  // bytes of rows
   g4_problem p;             // of a step
   int per;                  // sequences of a step
@@ -1018,7 +1023,7 @@ struct CacheExpand {
     const int64_t one = most * hkv * d * 4;  // K and V of a sequence
     const int64_t fit = std::min(kMost / one, (int64_t)0x7fffffff / std::max<int64_t>(most, a.max_seqlen_q));
     per = (int)std::min<int64_t>(a.table.batch, std::max<int64_t>(1, fit));
-    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(d) &&
+    used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(a) &&
            (int64_t)hkv * d < (int64_t(1) << 24) &&
            (most * per / 32 + per) * hkv <= 0x7fffffffLL;
     operand = align256((size_t)most * per * hkv * d * 2);

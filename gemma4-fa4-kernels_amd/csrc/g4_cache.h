@@ -130,8 +130,11 @@ struct CacheAttnParams {
   float* lse;
   g4_layout ql, ol;
   // Set by the launcher (g4_cache_attn.hip): workgroups at most, groups and queries of
-  // a set; the parts' heads, and their sums of the segments that several parts share.
-  int parts, set_groups, set_queries;
+  // a set, tiles that a workgroup takes at once, whether it is the wide kernel's,
+  // (sequence, set, KV head) segments at most; the parts' heads, and their sums of the
+  // segments that several parts share.
+  int parts, set_groups, set_queries, step_tiles, wide;
+  int64_t segments;
   struct PartHead* heads;
   float* part;
 };

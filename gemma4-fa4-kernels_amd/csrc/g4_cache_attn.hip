@@ -16,7 +16,7 @@
 //
 // One, two or four groups (a set) share a workgroup of four waves, which then take
 // the set's tiles side by side, so that a tile comes from memory once for up to 64
-// rows.  The tiles of all (sequence, set, KV head) segments, in that order, are cut
+// rows (at head dim 512 more than one group go to cache_wide_kernel).  The tiles of all (sequence, set, KV head) segments, in that order, are cut
 // into equal parts, one workgroup each, so that the longest sequence of a batch
 // does not decide its time.  A group's waves take its tiles in turn and add up
 // through LDS; a segment inside one part is finished there, else the parts' sums go
@@ -142,8 +142,11 @@ struct PartStart {
   CacheSeq seq;  // sequence s
 };
 __device__ __forceinline__ int part_count(const CacheAttnParams& a, int64_t tiles) {
-  // (each of a set's groups has kWaves / sets waves: at least a tile for each)
-  return (int)max(min((int64_t)a.parts, tiles / (kWaves / a.set_groups)), (int64_t)(tiles > 0));
+  // A part has as many tiles as its waves take at once, or, of segments shorter than
+  // that, one segment: one after the other they cost a chain of loads each (4 sequences
+  // of 2 tokens, 4 heads of 512: 43 us four to a part, 18 so).
+  const int64_t n = max(tiles / a.step_tiles, min(tiles, a.segments));
+  return (int)min((int64_t)a.parts, n);
 }
 __device__ __forceinline__ int part_of(int64_t x, int parts, int64_t tiles) {
   return (int)(((x + 1) * parts - 1) / tiles);
@@ -216,6 +219,56 @@ static_assert(sizeof(PartHead) == 40, "a part's head");
 __device__ __forceinline__ int64_t part_slot(int part, int64_t part_lo, int64_t seg0) {
   return 2 * (int64_t)part + (seg0 > part_lo);
 }
+
+// The segments of a part in order: the one at hand, and the part's share of its tiles.
+struct PartWalk {
+  int64_t lo, hi, seg0;  // the part's tiles that are left, the segment's first tile
+  int s, set, kvh;
+  CacheSeq sq;  // sequence s
+  TileRange range;
+  __device__ __forceinline__ void set_range(const CacheAttnParams& a) {
+    range.init(a, sq, set * a.set_queries, min((set + 1) * a.set_queries, sq.lq) - 1);
+  }
+  __device__ __forceinline__ void init(const CacheAttnParams& a, const PartStart& f) {
+    lo = f.lo;
+    hi = f.hi;
+    seg0 = f.seq0;
+    s = f.s;
+    sq = f.seq;
+    const int hkv = a.c.num_kv_heads;
+    for (set = 0;; ++set) {
+      set_range(a);
+      const int64_t n = (int64_t)range.n * hkv;
+      if (lo < seg0 + n) break;
+      seg0 += n;
+    }
+    kvh = (int)((lo - seg0) / range.n);
+    seg0 += (int64_t)kvh * range.n;
+  }
+  __device__ __forceinline__ int x0() const { return (int)(lo - seg0); }
+  __device__ __forceinline__ int x1() const { return (int)min(hi - seg0, (int64_t)range.n); }
+  __device__ __forceinline__ PartHead head(const CacheAttnParams& a, const PartStart& f) const {
+    const int gsh = __builtin_ctz(a.num_q_heads / a.c.num_kv_heads);
+    return {f.tiles, seg0, f.parts, range.n, kvh, sq.q0 + set * a.set_queries,
+            min(a.set_queries, sq.lq - set * a.set_queries) << gsh, 0};
+  }
+  // False: the part has no further segment.
+  __device__ __forceinline__ bool next(const CacheAttnParams& a) {
+    lo = seg0 + range.n;
+    if (lo >= hi) return false;
+    seg0 = lo;
+    if (++kvh == a.c.num_kv_heads) {
+      kvh = 0;
+      ++set;
+      while (set * a.set_queries >= sq.lq) {  // (tiles are left, so sequences are)
+        sq.init(a, ++s);
+        set = 0;
+      }
+      set_range(a);
+    }
+    return true;
+  }
+};
 
 template <int D>
 struct CacheWave {
@@ -355,30 +408,17 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
     if (part == 0 && tid == 0) a.heads[0].parts = 0;
     return;
   }
-  int64_t lo = f.lo;
-  const int64_t hi = f.hi;
-  int s = f.s;
-  CacheSeq sq = f.seq;
-  int64_t seg0 = f.seq0;  // first tile of the segment at hand
-  int set = 0, kvh = 0;
-  TileRange range;
-  for (;; ++set) {
-    range.init(a, sq, set * a.set_queries, min((set + 1) * a.set_queries, sq.lq) - 1);
-    const int64_t n = (int64_t)range.n * hkv;
-    if (lo < seg0 + n) break;
-    seg0 += n;
-  }
-  kvh = (int)((lo - seg0) / range.n);
-  seg0 += (int64_t)kvh * range.n;
+  PartWalk walk;
+  walk.init(a, f);
+  if (tid == 0) a.heads[part] = walk.head(a, f);
   const int grp = a.num_q_heads / hkv, gsh = __builtin_ctz(grp);
-  if (tid == 0)
-    a.heads[part] = PartHead{f.tiles, seg0, f.parts, range.n, kvh,
-                             sq.q0 + set * a.set_queries,
-                             min(a.set_queries, sq.lq - set * a.set_queries) << gsh, 0};
   const int blocks = a.c.page_size / kTile;
-  while (true) {
+  do {
     // ---- the part's share [x0, x1) of the segment's tiles ---------------------
-    const int x0 = (int)(lo - seg0), x1 = (int)min(hi - seg0, (int64_t)range.n);
+    const CacheSeq& sq = walk.sq;
+    const TileRange& range = walk.range;
+    const int kvh = walk.kvh, set = walk.set;
+    const int x0 = walk.x0(), x1 = walk.x1();
     const int set_first = set * a.set_queries;
     const int set_last = min(set_first + a.set_queries, sq.lq) - 1;
     const int q_first = set_first + sub * (kGroupRows >> gsh);  // of this wave's group
@@ -388,7 +428,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
     const int head = kvh * grp + (i & (grp - 1));
     const bool valid = my_q <= q_last;
     const int a_row = valid ? my_q + off : -1;
-    const int* const pages = a.tab.pages + (int64_t)s * a.tab.width;
+    const int* const pages = a.tab.pages + (int64_t)walk.s * a.tab.width;
 
     W w;
     {
@@ -471,7 +511,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
     const bool whole = x0 == 0 && x1 == range.n;
     const int nrows = (set_last - set_first + 1) << gsh;
     float* const part_o =
-        a.part + part_slot(part, f.lo, seg0) * (int64_t)(sets * kGroupRows * (D + 2));
+        a.part + part_slot(part, f.lo, walk.seg0) * (int64_t)(sets * kGroupRows * (D + 2));
     constexpr int kCols = D / 4;  // threads of a row, four elements each
     for (int r = tid / kCols; r < nrows; r += 256 / kCols) {
       const int d = tid % kCols * 4, g = r / kGroupRows, ri = r % kGroupRows;
@@ -504,27 +544,323 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 1) cache_attn_kernel(Cache
         }
       }
     }
+  } while (walk.next(a));
+}
 
-    // ---- the next segment ------------------------------------------------------
-    lo = seg0 + range.n;
-    if (lo >= hi) break;
-    seg0 = lo;
-    if (++kvh == hkv) {
-      kvh = 0;
-      ++set;
-      while (set * a.set_queries >= sq.lq) {  // (tiles are left, so sequences are)
-        sq.init(a, ++s);
-        set = 0;
-      }
-      range.init(a, sq, set * a.set_queries, min((set + 1) * a.set_queries, sq.lq) - 1);
-    }
+// ---------------------------------------------------------------------------
+// More rows of a KV head than 16, head dim 512: a set of 16 G rows in one workgroup,
+// which takes 64 keys (two tiles) a step.  A wave scores 16 of the keys against all
+// rows (Q from LDS, in the order of the operand), then adds 128 of the columns of V for
+// all keys and rows, so that each element of K and V is converted once for the whole
+// set.  Between the two P^T goes through LDS: the scores of a lane are 4 of the 8
+// elements of the same lane's operand.  All waves keep the rows' maxima; each has its
+// keys' share of their sums and whole sums of its columns.
+//
+// Between HBM (64 KB a step and CU: 3.2 us) and what G costs a step (16 + 16 matrix
+// instructions, 64 KB of Q from LDS and a softmax a group: 0.8 us).  Whole calls with
+// this kernel / with the one above, a wave a tile and 16 rows: 2 x 100000 tokens, 5 new
+// (G = 3) 184 / 351 us, 8 x 8000, 3, 6 and 8 new 56 / 77, 72 / 117 and 85 / 133.  Loads
+// are a step ahead, the table's entries two: with the entries one step ahead 212 us for
+// the first (each step waits for them and, in order, for the values before them).
+// ---------------------------------------------------------------------------
+template <int G>
+__global__ void __launch_bounds__(256, 1) cache_wide_kernel(CacheAttnParams a) {
+  constexpr int D = 512;
+  constexpr int kNC = D / 64;               // 16-byte chunks of a lane's K row
+  constexpr int kCols = D / kWaves;         // columns of a wave
+  constexpr int kNB = kCols / 16;           // its O^T blocks
+  constexpr int kRows = G * kGroupRows;
+  __shared__ u32x4 qs[G][2 * kNC][64];      // operands of Q
+  __shared__ u32x2 ps[2][G][64][2];         // operands of P^T: [tile][group][lane][half]
+  __shared__ f32x4 stat[kRows];             // a value of each wave per row
+  __shared__ int64_t scan[kWaves + 2];
+  const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int own = wave >> 1, half = wave & 1;  // the tile of the step and its keys to score
+  const int hkv = a.c.num_kv_heads;
+
+  const int part = blockIdx.x;
+  PartStart f;
+  if (!find_part(a, part, (int64_t G4_LDS*)scan, f)) {
+    if (part == 0 && tid == 0) a.heads[0].parts = 0;
+    return;
   }
+  PartWalk w;
+  w.init(a, f);
+  if (tid == 0) a.heads[part] = w.head(a, f);
+  const int grp = a.num_q_heads / hkv, gsh = __builtin_ctz(grp);
+  const int blocks = a.c.page_size / kTile;
+  do {
+    const int x0 = w.x0(), x1 = w.x1();
+    const int set_first = w.set * a.set_queries;
+    const int set_last = min(set_first + a.set_queries, w.sq.lq) - 1;
+    const int off = w.sq.len - w.sq.lq;
+    const int nrows = (set_last - set_first + 1) << gsh;
+    const int* const pages = a.tab.pages + (int64_t)w.s * a.tab.width;
+
+    // ---- Q (rows past the set's: its first, whose results are dropped) ----------------
+    constexpr int kMine = 2 * kNC / kWaves;  // this wave's operands of a group
+    u32x4 q[G][kMine];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int row = g * kGroupRows + i, r = row < nrows ? row : 0;
+      const __bf16* src = a.q + (int64_t)(w.sq.q0 + set_first + (r >> gsh)) * a.ql.token_stride +
+                          (int64_t)(w.kvh * grp + (r & (grp - 1))) * a.ql.head_stride + 16 * h;
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) {
+        const int st = wave * kMine + n;
+        q[g][n] = *(const u32x4*)(src + 64 * (st >> 1) + 8 * (st & 1));
+      }
+    }
+
+    u32x4 k[kNC];     // key i of this wave's half tile
+    u32x2 v[2][8];    // keys 16 (j >> 2) + 4 h + (j & 3) of both tiles, columns 8 i + 0..7
+    float ks, vs[2];
+    int t[2], id[2];  // a step's tiles and their pages, or -1
+    int tn[2], entry[2];  // the next step's, whose table entries are on their way
+    // (a tile without a page is read from page 0 and masked: no branch around the loads)
+    auto fetch = [&](int x) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        tn[b] = x + b < x1 ? w.range.at(x + b) : -1;
+        entry[b] = pages[min(max(tn[b], 0) * kTile / a.c.page_size, a.tab.width - 1)];
+      }
+    };
+    auto resolve = [&]() {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        t[b] = tn[b];
+        const int page = __builtin_amdgcn_readfirstlane(entry[b]);
+        id[b] = t[b] >= 0 && t[b] * kTile / a.c.page_size < a.tab.width &&
+                        (unsigned)page < (unsigned)a.c.num_pages
+                    ? page
+                    : -1;
+      }
+    };
+    auto load_k = [&]() {
+      const int64_t p = uniform((int64_t)max(own ? id[1] : id[0], 0) * hkv + w.kvh);
+      const int blk = max(own ? t[1] : t[0], 0) % blocks;
+      const uint8_t* src = (const uint8_t*)a.c.k +
+                           (p * a.c.page_size + blk * kTile + 16 * half + i) * D + 16 * h;
+      ks = a.c.k_scale[p * blocks + blk];
+#pragma unroll
+      for (int c = 0; c < kNC; ++c) k[c] = *(const u32x4*)(src + c * 64);
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int64_t p = uniform((int64_t)max(id[b], 0) * hkv + w.kvh);
+        const int blk = max(t[b], 0) % blocks;
+        const uint8_t* src = (const uint8_t*)a.c.v +
+                             (p * a.c.page_size + blk * kTile + 4 * h) * D + wave * kCols + 8 * i;
+        vs[b] = a.c.v_scale[p * blocks + blk];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[b][j] = *(const u32x2*)(src + (16 * (j >> 2) + (j & 3)) * D);
+      }
+    };
+
+    f32x4 o[G][kNB];
+    float m[G], l[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      m[g] = kNegInf;
+      l[g] = 0.f;
+#pragma unroll
+      for (int b = 0; b < kNB; ++b) o[g][b] = f32x4{};
+    }
+    fetch(x0);
+    resolve();
+    // (in the loop's order, which its waits count)
+    load_k();
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(x0 + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) qs[g][wave * kMine + n][lane] = q[g][n];
+    barrier_lds();
+    for (int x = x0; x < x1; x += 2) {
+      // ---- scores of 16 keys -------------------------------------------------------
+      const int now[2] = {t[0], t[1]};
+      const bool there[2] = {id[0] >= 0, id[1] >= 0};
+      const bool page = own ? there[1] : there[0];
+      const int my_t = own ? now[1] : now[0];
+      f32x4 s[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[g] = f32x4{};
+      // (Q two steps ahead, K one, in this order: two reads in flight cost 1.2 us a step)
+      u32x4 qr[3][G];
+      auto read_q = [&](int st) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) qr[st % 3][g] = qs[g][st][lane];
+      };
+      auto key = [&](int st) -> bf16x8 {
+        const uint32_t k0 = k[st >> 1][2 * (st & 1)], k1 = k[st >> 1][2 * (st & 1) + 1];
+        return __builtin_bit_cast(bf16x8, u32x4{e4m3_pair<false>(k0, ks), e4m3_pair<true>(k0, ks),
+                                                e4m3_pair<false>(k1, ks), e4m3_pair<true>(k1, ks)});
+      };
+      read_q(0);
+      read_q(1);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 kf = key(0);
+#pragma unroll
+      for (int st = 0; st < 2 * kNC; ++st) {
+        if (st + 2 < 2 * kNC) read_q(st + 2);
+        const bf16x8 kn = key(min(st + 1, 2 * kNC - 1));
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          s[g] = mfma16(kf, __builtin_bit_cast(bf16x8, qr[st % 3][g]), s[g]);
+        kf = kn;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      resolve();
+      load_k();
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(x + 4);
+      __builtin_amdgcn_sched_barrier(0);
+      // (a tile past the part's share is masked whole)
+      const int kb0 = my_t * kTile + 16 * half;
+      if (!page || kb0 + 15 > set_first + off) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int row = g * kGroupRows + i;
+          const int a_row =
+              my_t >= 0 && row < nrows ? set_first + (row >> gsh) + off : -0x7fffffff;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[g][r] = kb0 + 4 * h + r <= a_row ? (page ? s[g][r] : __builtin_nanf("")) : kNegInf;
+        }
+      }
+      // ---- the rows' maxima over the waves -----------------------------------------
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float mx = rows_max(fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3])));
+        if (h == 0) ((float*)&stat[g * kGroupRows + i])[wave] = mx;
+      }
+      barrier_lds();
+      float alpha[G];
+      bool moved = false;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const f32x4 all = stat[g * kGroupRows + i];
+        const float mx = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])) * kLog2e;
+        // (moves only when exceeded by more than 2^8, as in CacheWave::softmax)
+        const float m_new = mx > m[g] + 8.f ? mx : m[g];
+        const float m_use = m_new == kNegInf ? 0.f : m_new;
+        alpha[g] = fast_exp2(m[g] - m_use);
+        float sum = 0.f;
+        bf16x4 pb;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = fast_exp2(__builtin_fmaf(s[g][r], kLog2e, -m_use));
+          sum += p;
+          pb[r] = (__bf16)p;
+        }
+        l[g] = l[g] * alpha[g] + sum;
+        m[g] = m_new;
+        moved |= alpha[g] != 1.f;
+        ps[own][g][lane][half] = __builtin_bit_cast(u32x2, pb);
+      }
+      if (__ballot(moved)) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int b = 0; b < kNB; ++b) o[g][b] *= alpha[g];
+      }
+      barrier_lds();
+      // ---- O^T += V^T P^T of 128 columns --------------------------------------------
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (!there[b]) continue;
+        if ((now[b] + 1) * kTile > w.sq.len) {
+          // rows past the sequence's end hold anything: as zeros
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (now[b] * kTile + 16 * (j >> 2) + 4 * h + (j & 3) >= w.sq.len) v[b][j] = u32x2{};
+        }
+        bf16x8 pb[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) pb[g] = *(const bf16x8*)&ps[b][g][lane][0];
+#pragma unroll
+        for (int y2 = 0; y2 < 2; ++y2) {
+          uint32_t lo[8], hi[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            lo[j] = e4m3_pair<false>(v[b][j][y2], vs[b]);
+            hi[j] = e4m3_pair<true>(v[b][j][y2], vs[b]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t* y = e < 2 ? lo : hi;
+            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+            u32x4 vf;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vf[j] = __builtin_amdgcn_perm(y[2 * j + 1], y[2 * j], sel);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              o[g][4 * y2 + e] = mfma16(__builtin_bit_cast(bf16x8, vf), pb[g], o[g][4 * y2 + e]);
+          }
+        }
+      }
+      load_v();
+    }
+
+    // ---- O and LSE, or the part's sums --------------------------------------------------
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float sum = rows_sum(l[g]);
+      if (h == 0) ((float*)&stat[g * kGroupRows + i])[wave] = sum;
+    }
+    barrier_lds();
+    const bool whole = x0 == 0 && x1 == w.range.n;
+    float* const part_o = a.part + part_slot(part, f.lo, w.seg0) * (int64_t)(kRows * (D + 2));
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int row = g * kGroupRows + i;
+      if (row >= nrows) continue;
+      const f32x4 all = stat[row];
+      const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+      // columns kCols wave + 8 (4 h + r) + 0..7
+      const int col = kCols * wave + 32 * h;
+      if (whole) {
+        const int qi = w.sq.q0 + set_first + (row >> gsh), qh = w.kvh * grp + (row & (grp - 1));
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays)
+        __bf16* const out = a.o + (int64_t)qi * a.ol.token_stride + (int64_t)qh * a.ol.head_stride + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          bf16x8 y;
+#pragma unroll
+          for (int b = 0; b < kNB; ++b) y[b] = (__bf16)(o[g][b][r] * inv);
+          *(bf16x8*)(out + 8 * r) = y;
+        }
+        if (wave == 0 && h == 0)
+          a.lse[(int64_t)qh * a.total_q + qi] =
+              sum == 0.f ? kNegInf : (m[g] + fast_log2(sum)) * kLn2;
+      } else {
+        float* const out = part_o + row * D + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          *(f32x4*)(out + 8 * r) = f32x4{o[g][0][r], o[g][1][r], o[g][2][r], o[g][3][r]};
+          *(f32x4*)(out + 8 * r + 4) = f32x4{o[g][4][r], o[g][5][r], o[g][6][r], o[g][7][r]};
+        }
+        if (wave == 0 && h == 0) {
+          float* const ml = part_o + kRows * D + 2 * row;
+          ml[0] = m[g];
+          ml[1] = sum;
+        }
+      }
+    }
+  } while (w.next(a));
 }
 
 // O and LSE of the segments that more than one part holds.  The workgroup of part w
 // serves the segment that part w begins inside of, as one of the n - 1 workgroups
-// whose parts do: each takes an equal run of the rows' elements, four a thread, and
-// where those are fewer than the threads, several threads share the parts.
+// whose parts do (gridDim.y for each): each takes an equal run of the rows' elements,
+// four a thread, and where those are fewer than the threads, several threads share the
+// parts.
 template <int D>
 __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
   __shared__ __attribute__((aligned(16))) float acc_lds[256][4];
@@ -548,8 +884,8 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
   const auto sums = [&](int c) { return c == 0 ? part0 : part1 + 2 * (int64_t)(c - 1) * slot; };
 
   const int units = hd.rows * (D / 4);  // four elements of a row each
-  const int u0 = (int)((int64_t)units * (w - w0 - 1) / (n - 1));
-  const int u1 = (int)((int64_t)units * (w - w0) / (n - 1));
+  const int y = gridDim.y * (w - w0 - 1) + blockIdx.y, ny = gridDim.y * (n - 1);
+  const int u0 = (int)((int64_t)units * y / ny), u1 = (int)((int64_t)units * (y + 1) / ny);
   int subs = 1;  // threads of a unit
   while (subs < 16 && subs * 2 * (u1 - u0) <= 256) subs *= 2;
   const int per = 256 / subs;
@@ -624,13 +960,20 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
 // Workgroups that are resident at once.
 static int cache_parts(int head_dim) { return head_dim == 256 ? 512 : 256; }
 
-// Groups of a set: as many as the batch's longest run of new tokens fills.
+// Groups of a set: as many as the batch's longest run of new tokens fills, up to what
+// a kernel takes, in sets of about equal rows.
 static void cache_sets(CacheAttnParams* a) {
   const int grp = a->num_q_heads / a->c.num_kv_heads;
-  const int64_t rows = (int64_t)a->max_q * grp;
-  a->set_groups = rows <= kGroupRows ? 1 : rows <= 2 * kGroupRows ? 2 : 4;
+  const int64_t groups = ((int64_t)a->max_q * grp + kGroupRows - 1) / kGroupRows;
+  a->wide = a->c.head_dim == 512 && groups > 1;
+  const int64_t sets = (groups + 3) / 4;
+  const int n = (int)((groups + sets - 1) / sets);
+  a->set_groups = !a->wide && n == 3 ? 4 : n;
   a->set_queries = a->set_groups * kGroupRows / grp;
   a->parts = cache_parts(a->c.head_dim);
+  a->step_tiles = a->wide ? 2 : kWaves / a->set_groups;
+  a->segments = (int64_t)a->tab.batch * a->c.num_kv_heads *
+                ((a->max_q + a->set_queries - 1) / a->set_queries);
 }
 
 static size_t heads_bytes(const CacheAttnParams& a) {
@@ -642,12 +985,24 @@ size_t cache_part_bytes(CacheAttnParams a) {
   return heads_bytes(a) + (size_t)2 * a.parts * a.set_groups * kGroupRows * (a.c.head_dim + 2) * 4;
 }
 
+// Workgroups of the merge for a cut: 26 sequences of 12 new tokens (sets of 48 rows) 158
+// us in all with one, 147 with three, 142 with six; 5 of 15 20.4, 17.7 and 21.9.
+static int merge_blocks(int set_groups) { return set_groups; }
+
 template <int D>
 static hipError_t launch_cache_attn_d(const CacheAttnParams& a, hipStream_t stream) {
-  hipLaunchKernelGGL(cache_attn_kernel<D>, dim3((unsigned)a.parts), dim3(256), 0, stream, a);
+  void (*kern)(CacheAttnParams) = cache_attn_kernel<D>;
+  if constexpr (D == 512)
+    if (a.wide)
+      kern = a.set_groups == 2   ? cache_wide_kernel<2>
+             : a.set_groups == 3 ? cache_wide_kernel<3>
+                                 : cache_wide_kernel<4>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.parts), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(cache_merge_kernel<D>, dim3((unsigned)a.parts - 1), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(cache_merge_kernel<D>,
+                     dim3((unsigned)a.parts - 1, (unsigned)merge_blocks(a.set_groups)), dim3(256),
+                     0, stream, a);
   return hipGetLastError();
 }
 

@@ -251,8 +251,8 @@ def paged_cache_attention(
     window nor sinks; query heads are 1, 2, 4 or 8 times the cache's.
 
     A few new tokens per sequence are computed from the pages as they lie; from more
-    than 128 query rows per KV head on (192 at head dim 256), what the batch can see is
-    laid out as bf16 rows in a workspace (``4 * tokens * Hkv * head_dim`` bytes a
+    than 448 query rows per KV head on (192 at head dim 256, 320 of one or two
+    sequences), what the batch can see is laid out as bf16 rows in a workspace (``4 * tokens * Hkv * head_dim`` bytes a
     sequence, as many sequences at a time as fit 8 GiB).
     """
     desc = cache.descriptor()

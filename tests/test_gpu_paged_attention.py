@@ -347,3 +347,62 @@ def test_a_window_past_every_length(window):
         got = attend(q, cache, table, lens, new, window=window, sinks=3)
         check_attention(q, cache, table, lens, new, *got)
         assert torch.equal(torch.isneginf(got[1]), torch.isneginf(want[1]))
+
+
+# Sets of 2, 3 and 4 groups of 16 rows a workgroup, each with a last one that is part full,
+# steps of two tiles that end inside one and in the first, and several sets.
+@pytest.mark.parametrize("hkv,grp,page,lens,new", [
+    (1, 8, 32, [700, 100], [6, 2]),
+    (2, 8, 64, [500], [56]),  # 448 rows, the most that are read as they lie
+    (2, 8, 64, [500], [57]),
+    (1, 2, 64, [300, 64], [24, 9]),
+    (1, 1, 64, [200, 33], [48, 17]),
+    (4, 8, 128, [3001, 70, 5], [10, 2, 5]),
+    (2, 4, 256, [90000], [13]),
+    (1, 8, 32, [31 + b for b in range(70)], [1 + b % 4 for b in range(70)]),
+])
+def test_sets_of_rows_at_head_dim_512(hkv, grp, page, lens, new):
+    run(lens[0] + new[0], 512, hkv, grp, page, lens, new)
+    run(lens[0] + new[0], 512, hkv, grp, page, lens, new, max_q=max(new) + 3, max_k=max(lens) + 9)
+
+
+def test_large_scores_of_a_set():
+    cache, table = filled_cache(31, [2000], 1, 64, 512, std_k=4.0)
+    q = queries(31, 7, 8, 512, scale=30.0)
+    out, lse = attend(q, cache, table, [2000], [7])
+    check_attention(q, cache, table, [2000], [7], out, lse)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [9, 2], [40, 61]])
+def test_what_lies_past_the_end_is_not_seen_at_head_dim_512(new):
+    lens = [333, 61]
+    clean, table = filled_cache(32, lens, 2, 32, 512)
+    q = queries(32, sum(new), 8, 512)
+    want = attend(q, clean, table, lens, new)
+    cache, _ = filled_cache(32, lens, 2, 32, 512)
+    used = torch.zeros(cache.num_pages, 32, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            used[table[b][t // 32], t % 32] = True
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).masked_fill_(~used.to(DEV)[:, None, :, None], 0x7F)
+    for t in (cache.k_scale, cache.v_scale):
+        t.masked_fill_(~used.any(1).to(DEV)[:, None, None], float("nan"))
+    got = attend(q, cache, table, lens, new)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_a_set_and_a_token_without_a_page():
+    lens, new = [200, 100], [20, 9]
+    cache, table = filled_cache(33, lens, 2, 32, 512)
+    q = queries(33, 29, 8, 512)
+    want, want_lse = attend(q, cache, table, lens, new)
+    table[0][6] = -1  # tokens 192 .. 199: seen from position 192 on, query 12 of 20
+    got, lse = attend(q, cache, table, lens, new)
+    assert torch.equal(got[:12], want[:12]) and got[12:20].isnan().all()
+    assert torch.equal(got[20:], want[20:]) and torch.equal(lse[:, 20:], want_lse[:, 20:])
+
+
+@pytest.mark.parametrize("new", [160, 161])  # 320 rows, the most that are read as they lie
+def test_a_chunk_of_one_local_conversation(new):
+    run(34, 256, 2, 2, 64, [3000], [new], 1024, 4)
