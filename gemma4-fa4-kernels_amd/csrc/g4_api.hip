@@ -1021,7 +1021,8 @@ struct CacheExpand {
                                      : (int64_t)a.max_seqlen_k;
     const int64_t most = std::min<int64_t>(a.max_seqlen_k, see);
     const int64_t one = most * hkv * d * 4;  // K and V of a sequence
-    const int64_t fit = std::min(kMost / one, (int64_t)0x7fffffff / std::max<int64_t>(most, a.max_seqlen_q));
+    const int64_t rows = std::max<int64_t>(most, a.max_seqlen_q);
+    const int64_t fit = std::min(kMost / one, (int64_t)0x7fffffff / rows);
     per = (int)std::min<int64_t>(a.table.batch, std::max<int64_t>(1, fit));
     used = (int64_t)a.max_seqlen_q * (a.num_q_heads / hkv) > as_they_lie(a) &&
            (int64_t)hkv * d < (int64_t(1) << 24) &&

@@ -13,8 +13,9 @@ namespace g4 {
 // block's earlier tokens next to nothing, and what a block holds does not
 // depend on how its tokens were dealt to the calls but there.  Bound by HBM: a
 // row is read once (2 bytes an element) and written once (1 byte): 19500 tokens of 16
-// heads of 256 in 99 us, 4.8 TB/s (with the heads' rows apart in the grid 109).  One
-// token a sequence is a chain of latencies: 64 sequences 6.7 us.
+// heads of 256 in 98 us, 4.9 TB/s (with the heads' rows apart in the grid 109).  One
+// token a sequence is a chain of latencies: 64 sequences 5.6 us (6.7 with the table
+// read before the rows, and a sequence's length after its number).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
@@ -26,17 +27,14 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
   // heads first: neighbouring workgroups read neighbouring runs of the same rows
   const int head = blockIdx.x % c.num_kv_heads, slot = blockIdx.x / c.num_kv_heads;
   const int which = blockIdx.y;
-  const int s = find_sequence(a.cu, a.tab.batch, slot, 2);
-  const int row0 = a.cu[s], n = a.cu[s + 1] - row0;
-  const int len = a.tab.seq_lens[s];
+  const SequenceOf seq(a.cu, a.tab.seq_lens, a.tab.batch, slot, 2);
+  const int s = seq.s, row0 = seq.row0, n = seq.end - row0, len = seq.len;
   const int first = len - n;  // position of the first new token
   const int begin = max(first, 0);
   const int rel = slot - (row0 / 32 + 2 * s);
   if (n <= 0 || rel < 0 || len <= begin) return;
   const int64_t t0 = (int64_t)(begin / kCacheBlock + rel) * kCacheBlock;
   if (t0 >= len) return;
-  const int page = page_of(a.tab, c, s, (int)t0);
-  if (page < 0) return;
   const int lo = max(begin - (int)t0, 0), hi = min(len - (int)t0, kCacheBlock);
 
   const int tid = threadIdx.x, lane = tid & 63, sub = tid / kLanes, col = tid % kLanes;
@@ -50,6 +48,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams a) {
     if (r >= lo && r < hi && row >= 0 && row < a.total)
       x[i] = *(const u32x4*)(in + row * a.lay[which].token_stride);
   }
+  const int page = page_of(a.tab, c, s, (int)t0);  // (after the rows' loads: they overlap)
+  if (page < 0) return;
   // largest finite magnitude: bf16 bits without the sign compare as numbers do
   int most = 0;
 #pragma unroll
@@ -129,11 +129,11 @@ __global__ void __launch_bounds__(256) gather_kernel(GatherParams a) {
   const g4_paged_cache& c = a.c;
   const int head = blockIdx.x % c.num_kv_heads, slot = blockIdx.x / c.num_kv_heads;
   const int which = blockIdx.y;
-  const int s = find_sequence(a.cu, a.tab.batch, slot, 1);
-  const int row0 = a.cu[s], n = a.cu[s + 1] - row0;
+  const SequenceOf seq(a.cu, a.tab.seq_lens, a.tab.batch, slot, 1);
+  const int s = seq.s, row0 = seq.row0, n = seq.end - row0;
   const int rel = slot - (row0 / 32 + s);
   if (rel < 0 || rel >= (n + 31) / 32) return;
-  int len = a.tab.seq_lens[s], shift = 0;
+  int len = seq.len, shift = 0;
   if (a.cu_q != nullptr) {
     VisibleRows v;
     len = min(max(len, 0), a.max_k);

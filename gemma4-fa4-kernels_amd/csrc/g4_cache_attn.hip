@@ -16,13 +16,13 @@
 //
 // One, two or four groups (a set) share a workgroup of four waves, which then take
 // the set's tiles side by side, so that a tile comes from memory once for up to 64
-// rows (at head dim 512 more than one group go to cache_wide_kernel).  The tiles of all (sequence, set, KV head) segments, in that order, are cut
-// into equal parts, one workgroup each, so that the longest sequence of a batch
-// does not decide its time.  A group's waves take its tiles in turn and add up
-// through LDS; a segment inside one part is finished there, else the parts' sums go
-// to the workspace (two slots a part: only the segments it begins and ends in can be
-// cut), and the second launch has a workgroup for each cut: those of one segment
-// share its rows' elements evenly.
+// rows (head dim 512: more than one group go to cache_wide_kernel).  The tiles of all
+// (sequence, set, KV head) segments, in that order, are cut into equal parts, one
+// workgroup each, so that the longest sequence of a batch does not decide its time.  A
+// group's waves take its tiles in turn and add up through LDS; a segment inside one
+// part is finished there, else the parts' sums go to the workspace (two slots a part:
+// only the segments it begins and ends in can be cut), and the second launch has
+// workgroups for each cut: those of one segment share its rows' elements evenly.
 //
 // Bound by HBM for long batches (1 byte an element of K and V: 2 x 100000 tokens of 4
 // heads of 512 in 145 us, 5.4 TB/s; 16 of 4096 to 8192 tokens 89 + 6 us, of which about
@@ -313,9 +313,9 @@ struct CacheWave {
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const u32x4 w = {e4m3_pair<false>(k[u][c][2 * x], ks), e4m3_pair<true>(k[u][c][2 * x], ks),
-                           e4m3_pair<false>(k[u][c][2 * x + 1], ks),
-                           e4m3_pair<true>(k[u][c][2 * x + 1], ks)};
+          const uint32_t k0 = k[u][c][2 * x], k1 = k[u][c][2 * x + 1];
+          const u32x4 w = {e4m3_pair<false>(k0, ks), e4m3_pair<true>(k0, ks),
+                           e4m3_pair<false>(k1, ks), e4m3_pair<true>(k1, ks)};
           s[u] = mfma16(__builtin_bit_cast(bf16x8, w), q[2 * c + x], s[u]);
         }
   }
@@ -828,7 +828,8 @@ __global__ void __launch_bounds__(256, 1) cache_wide_kernel(CacheAttnParams a) {
       if (whole) {
         const int qi = w.sq.q0 + set_first + (row >> gsh), qh = w.kvh * grp + (row & (grp - 1));
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays)
-        __bf16* const out = a.o + (int64_t)qi * a.ol.token_stride + (int64_t)qh * a.ol.head_stride + col;
+        __bf16* const out =
+            a.o + (int64_t)qi * a.ol.token_stride + (int64_t)qh * a.ol.head_stride + col;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           bf16x8 y;

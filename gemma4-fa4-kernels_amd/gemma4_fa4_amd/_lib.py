@@ -227,10 +227,13 @@ def load(path: str | None = None) -> ctypes.CDLL:
         return lib
 
 
+_NO_SCOPE = contextlib.nullcontext()
+
+
 def device_scope(device: torch.device):
     """A guard that makes ``device`` current for a launch (none when it already is)."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _NO_SCOPE
     return torch.cuda.device(device)
 
 

@@ -112,8 +112,8 @@ class PagedKVCache:
 
 
 def _ints(t: torch.Tensor, shape, device, name: str) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be an INT32 tensor of shape {shape}")
+    if t.dtype != torch.int32 or t.shape != shape:
+        raise ValueError(f"{name} must be an INT32 tensor of shape {tuple(shape)}")
     if t.device != device:
         raise ValueError(f"{name} must share the cache's device")
     if not t.is_contiguous():
@@ -121,16 +121,26 @@ def _ints(t: torch.Tensor, shape, device, name: str) -> None:
 
 
 def _table(page_table: torch.Tensor, seq_lens: torch.Tensor | None, device) -> G4PageTable:
-    if page_table.ndim != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
         raise ValueError("page_table must be a rank-2 (batch, width) tensor")
-    if page_table.numel() > _INT32_MAX:
+    batch, width = shape
+    if batch * width > _INT32_MAX:
         raise UnsupportedMI355XPath("page_table must have fewer than 2^31 entries")
-    batch, width = page_table.shape
-    _ints(page_table, (batch, width), device, "page_table")
+    _ints(page_table, shape, device, "page_table")
     if seq_lens is None:
         return G4PageTable(page_table.data_ptr(), page_table.data_ptr(), batch, width)
     _ints(seq_lens, (batch,), device, "seq_lens")
     return G4PageTable(page_table.data_ptr(), seq_lens.data_ptr(), batch, width)
+
+
+def _rows_layout(t: torch.Tensor, name: str) -> G4Layout:
+    """The layout of packed rows (T, H, 256 or 512), checked."""
+    _, heads, head_dim = t.shape
+    strides = t.stride()
+    if strides != (heads * head_dim, head_dim, 1):  # (those of contiguous rows will do)
+        _validate_layout(t, name=name)
+    return G4Layout(0, strides[0], strides[1])
 
 
 def _window(sliding_window: int | None) -> int:
@@ -144,8 +154,8 @@ def _window(sliding_window: int | None) -> int:
     return min(sliding_window, _INT32_MAX)
 
 
-def _no_autograd(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_autograd(needed: bool) -> None:
+    if needed and torch.is_grad_enabled():
         raise UnsupportedMI355XPath("the paged cache cannot participate in autograd")
 
 
@@ -171,24 +181,22 @@ def paged_cache_append(
     desc = cache.descriptor()
     if k.ndim != 3 or v.ndim != 3 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("k and v must be rank-3 BF16 (T, H, D) tensors")
-    if k.shape[1:] != (cache.num_kv_heads, cache.head_dim) or v.shape != k.shape:
+    shape = k.shape
+    if shape[1] != cache.num_kv_heads or shape[2] != cache.head_dim or v.shape != shape:
         raise ValueError("k and v must match each other and the cache's heads and head dim")
     if k.device != cache.device or v.device != cache.device:
         raise ValueError("k and v must share the cache's device")
-    _no_autograd(k, v)
+    _no_autograd(k.requires_grad or v.requires_grad)
     table = _table(page_table, seq_lens, cache.device)
     _ints(cu_seqlens, (table.batch + 1,), cache.device, "cu_seqlens")
     if k.shape[0] == 0:
         return
-    _validate_layout(k, name="k")
-    _validate_layout(v, name="v")
+    k_layout, v_layout = _rows_layout(k, "k"), _rows_layout(v, "v")
     _check_real_operands((k, v), ("k", "v"), label="k and v")
     with _lib.device_scope(cache.device):
         _lib.check(_lib.load().g4_cache_append(
             ctypes.byref(desc), ctypes.byref(table), cu_seqlens.data_ptr(), k.shape[0],
-            k.data_ptr(), G4Layout(0, k.stride(0), k.stride(1)),
-            v.data_ptr(), G4Layout(0, v.stride(0), v.stride(1)),
-            _lib.raw_stream(cache.device)))
+            k.data_ptr(), k_layout, v.data_ptr(), v_layout, _lib.raw_stream(cache.device)))
 
 
 def paged_cache_gather(
@@ -280,14 +288,14 @@ def paged_cache_attention(
         raise ValueError("num_sinks needs a sliding_window")
     if head_dim == 512 and sliding_window is not None:
         raise UnsupportedMI355XPath("head dim 512 attends without a window and sinks")
-    _no_autograd(q)
+    _no_autograd(q.requires_grad)
     table = _table(page_table, seq_lens, cache.device)
     _ints(cu_seqlens_q, (table.batch + 1,), cache.device, "cu_seqlens_q")
     out = _empty_as(q)
     lse = torch.empty((heads, total), dtype=torch.float32, device=q.device)
     if total == 0:
         return out, lse
-    _validate_layout(q, name="q")
+    q_layout = _rows_layout(q, "q")
     _check_real_operands((q,), ("q",), label="q")
     lib = _lib.load()
     prob = G4CacheAttn(desc, table, cu_seqlens_q.data_ptr(), total, heads,
@@ -296,7 +304,7 @@ def paged_cache_attention(
     ws = torch.empty(lib.g4_cache_attn_workspace_bytes(ref), dtype=torch.uint8, device=q.device)
     with _lib.device_scope(q.device):
         _lib.check(lib.g4_cache_attn_fwd(
-            ref, q.data_ptr(), G4Layout(0, q.stride(0), q.stride(1)),
-            out.data_ptr(), G4Layout(0, out.stride(0), out.stride(1)), lse.data_ptr(),
+            ref, q.data_ptr(), q_layout, out.data_ptr(),
+            G4Layout(0, heads * head_dim, head_dim), lse.data_ptr(),
             ws.data_ptr(), ws.numel(), _lib.raw_stream(q.device)))
     return out, lse

@@ -85,8 +85,8 @@ def test_hundreds_of_sequences():
     run(5, 256, 1, 2, 32, lens, [1] * 600, 64, 3)
 
 
-# Chunks: more than 128 query rows per KV head (192 at head dim 256) are attended over bf16
-# rows in the workspace; shorter ones of these in several sets of rows.
+# Chunks: more than 448 query rows per KV head (192 at head dim 256, 320 of one or two
+# sequences) are attended over bf16 rows in the workspace; shorter ones in several sets of rows.
 @pytest.mark.parametrize("d,hkv,grp,page,lens,new,window,sinks", [
     (512, 4, 8, 64, [900, 9, 300], [500, 9, 0], 0, 0),
     (512, 4, 8, 64, [6000, 20], [17, 1], 0, 0),  # a prompt's end and a step in one batch
