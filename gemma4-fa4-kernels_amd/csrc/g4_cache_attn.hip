@@ -30,6 +30,8 @@
 // merge for short ones (one window of 1024 tokens, 16 heads of 256: 11.6 + 5.4 us).
 // With one workgroup per (segment, row) the merge took 14 and 23 us (8 sequences of 5
 // new tokens) in place of 6 and 4.4.
+#include <type_traits>
+
 #include "g4_cache.h"
 
 namespace g4 {
@@ -142,10 +144,18 @@ struct PartStart {
   CacheSeq seq;  // sequence s
 };
 __device__ __forceinline__ int part_count(const CacheAttnParams& a, int64_t tiles) {
-  // A part has as many tiles as its waves take at once, or, of segments shorter than
-  // that, one segment: one after the other they cost a chain of loads each (4 sequences
-  // of 2 tokens, 4 heads of 512: 43 us four to a part, 18 so).
-  const int64_t n = max(tiles / a.step_tiles, min(tiles, a.segments));
+  // Few tiles: one each, as segments or a segment's waves that follow one another cost a
+  // chain of loads each (4 heads of 512, us with four tiles or segments to a part / so:
+  // 4 sequences of 2 tokens 43 / 18, 8 of 100 30 / 19, 3 of 428 28 / 20).  More: as many
+  // tiles as a workgroup takes at once, and for one sequence, whose segments are alike, a
+  // whole number of parts per segment, so that a part holds one of them (without / so: 4
+  // heads of 512, 4000 tokens 29 / 22; a window of 1024, 16 heads of 256 19.8 / 16.0).
+  if (tiles <= a.parts) return (int)tiles;
+  int64_t n = max(tiles / a.step_tiles, min(tiles, a.segments));
+  if (a.tab.batch == 1 && n < a.parts && a.segments <= n) {
+    const unsigned seg = (unsigned)a.segments;
+    n = ((unsigned)n + seg - 1) / seg * seg;
+  }
   return (int)min((int64_t)a.parts, n);
 }
 __device__ __forceinline__ int part_of(int64_t x, int parts, int64_t tiles) {
@@ -887,64 +897,8 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
   const int units = hd.rows * (D / 4);  // four elements of a row each
   const int y = gridDim.y * (w - w0 - 1) + blockIdx.y, ny = gridDim.y * (n - 1);
   const int u0 = (int)((int64_t)units * y / ny), u1 = (int)((int64_t)units * (y + 1) / ny);
-  int subs = 1;  // threads of a unit
-  while (subs < 16 && subs * 2 * (u1 - u0) <= 256) subs *= 2;
-  const int per = 256 / subs;
-  for (int ub = u0; ub < u1; ub += per) {
-    const int u = ub + tid / subs, sub = tid % subs;
-    const bool mine = u < u1;
-    const int r = mine ? u / (D / 4) : 0, d = u % (D / 4) * 4;
-    const int ml = set_rows * D + 2 * r, po = r * D + d;
-    float mx = kNegInf, sum = 0.f;
-    f32x4 acc = {};
-    if (mine) {
-      // four parts at a time, their loads in flight together
-      for (int c0 = sub; c0 < n; c0 += 4 * subs) {
-        f32x2 ml4[4];
-        f32x4 o4[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int c = min(c0 + v * subs, n - 1);
-          const float* const part = sums(c);
-          ml4[v] = *(const f32x2*)(part + ml);
-          o4[v] = *(const f32x4*)(part + po);
-        }
-        float m_new = mx;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          if (c0 + v * subs < n) m_new = fmaxf(m_new, ml4[v][0]);
-        const float m_use = m_new == kNegInf ? 0.f : m_new;
-        const float alpha = fast_exp2(mx - m_use);
-        sum *= alpha;
-        acc *= alpha;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          if (c0 + v * subs < n) {
-            const float wt = fast_exp2(ml4[v][0] - m_use);
-            sum += wt * ml4[v][1];
-            acc += wt * o4[v];
-          }
-        mx = m_new;
-      }
-    }
-    if (subs > 1) {
-      __syncthreads();
-      *(f32x4*)acc_lds[tid] = acc;
-      ml_lds[tid][0] = mx;
-      ml_lds[tid][1] = sum;
-      __syncthreads();
-      if (sub != 0) continue;
-      for (int v = 1; v < subs; ++v) mx = fmaxf(mx, ml_lds[tid + v][0]);
-      const float m_use = mx == kNegInf ? 0.f : mx;
-      sum = 0.f;
-      acc = f32x4{};
-      for (int v = 0; v < subs; ++v) {
-        const float wt = fast_exp2(ml_lds[tid + v][0] - m_use);
-        sum += wt * ml_lds[tid + v][1];
-        acc += wt * *(const f32x4*)acc_lds[tid + v];
-      }
-    }
-    if (!mine) continue;
+  const auto store = [&](int u, float mx, float sum, f32x4 acc) {
+    const int r = u / (D / 4), d = u % (D / 4) * 4;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int qrow = hd.q_row + (r >> gsh), qh = hd.kvh * grp + (r & (grp - 1));
     *(bf16x4*)(a.o + (int64_t)qrow * a.ol.token_stride + (int64_t)qh * a.ol.head_stride +
@@ -953,7 +907,91 @@ __global__ void __launch_bounds__(256) cache_merge_kernel(CacheAttnParams a) {
     if (d == 0)
       a.lse[(int64_t)qh * a.total_q + qrow] =
           sum == 0.f ? kNegInf : (mx + fast_log2(sum)) * kLn2;
+  };
+  // U units' sums over the parts c0, c0 + step, ..., C parts at a time, so that the loads
+  // of U x C are in flight together.
+  const auto add = [&](auto units_at_once, auto parts_at_once, const int* u, int c0, int step,
+                       float* mx, float* sum, f32x4* acc) {
+    constexpr int U = decltype(units_at_once)::value, C = decltype(parts_at_once)::value;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mx[i] = kNegInf, sum[i] = 0.f, acc[i] = f32x4{};
+    for (; c0 < n; c0 += C * step) {
+      f32x2 ml[C][U];
+      f32x4 o[C][U];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float* const part = sums(min(c0 + c * step, n - 1));
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int r = u[i] / (D / 4), d = u[i] % (D / 4) * 4;
+          ml[c][i] = *(const f32x2*)(part + set_rows * D + 2 * r);
+          o[c][i] = *(const f32x4*)(part + r * D + d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        float m_new = mx[i];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c0 + c * step < n) m_new = fmaxf(m_new, ml[c][i][0]);
+        const float m_use = m_new == kNegInf ? 0.f : m_new;
+        const float alpha = fast_exp2(mx[i] - m_use);
+        sum[i] *= alpha;
+        acc[i] *= alpha;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c0 + c * step < n) {
+            const float wt = fast_exp2(ml[c][i][0] - m_use);
+            sum[i] += wt * ml[c][i][1];
+            acc[i] += wt * o[c][i];
+          }
+        mx[i] = m_new;
+      }
+    }
+  };
+  // a thread a unit, up to four of them at a time
+  const auto each = [&](auto units_at_once, auto parts_at_once) {
+    constexpr int U = decltype(units_at_once)::value;
+    for (int ub = u0; ub < u1; ub += U * 256) {
+      int u[U];
+      float mx[U], sum[U];
+      f32x4 acc[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) u[i] = min(ub + i * 256 + tid, u1 - 1);
+      add(units_at_once, parts_at_once, u, 0, 1, mx, sum, acc);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (ub + i * 256 + tid < u1) store(u[i], mx[i], sum[i], acc[i]);
+    }
+  };
+  std::integral_constant<int, 1> one;
+  std::integral_constant<int, 2> two;
+  std::integral_constant<int, 4> four;
+  if (u1 - u0 > 512) return each(four, two);
+  if (u1 - u0 > 256) return each(two, four);
+  if (u1 - u0 > 128) return each(one, four);
+  int subs = 2;  // threads of a unit
+  while (subs < 16 && subs * 2 * (u1 - u0) <= 256) subs *= 2;
+  const int u = u0 + tid / subs, sub = tid % subs;
+  float mx, sum;
+  f32x4 acc;
+  const int at = min(u, max(u1 - 1, 0));
+  add(one, four, &at, sub, subs, &mx, &sum, &acc);
+  *(f32x4*)acc_lds[tid] = acc;
+  ml_lds[tid][0] = mx;
+  ml_lds[tid][1] = sum;
+  __syncthreads();
+  if (sub != 0 || u >= u1) return;
+  for (int v = 1; v < subs; ++v) mx = fmaxf(mx, ml_lds[tid + v][0]);
+  const float m_use = mx == kNegInf ? 0.f : mx;
+  sum = 0.f;
+  acc = f32x4{};
+  for (int v = 0; v < subs; ++v) {
+    const float wt = fast_exp2(ml_lds[tid + v][0] - m_use);
+    sum += wt * ml_lds[tid + v][1];
+    acc += wt * *(const f32x4*)acc_lds[tid + v];
   }
+  store(u, mx, sum, acc);
 }
 
 // ---- launches -------------------------------------------------------------------
