@@ -27,7 +27,7 @@
 // Bound by HBM for long batches (1 byte an element of K and V: 2 x 100000 tokens of 4
 // heads of 512 in 145 us, 5.4 TB/s; 16 of 4096 to 8192 tokens 89 + 6 us, of which about
 // 8 are the way to the first tile), by the chain of launch, lengths, table, page and
-// merge for short ones (one window of 1024 tokens, 16 heads of 256: 11.6 + 5.4 us).
+// merge for short ones (one window of 1024 tokens, 16 heads of 256: 9.5 + 5.8 us).
 // With one workgroup per (segment, row) the merge took 14 and 23 us (8 sequences of 5
 // new tokens) in place of 6 and 4.4.
 #include <type_traits>
