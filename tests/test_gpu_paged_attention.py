@@ -406,3 +406,40 @@ def test_a_set_and_a_token_without_a_page():
 @pytest.mark.parametrize("new", [160, 161])  # 320 rows, the most that are read as they lie
 def test_a_chunk_of_one_local_conversation(new):
     run(34, 256, 2, 2, 64, [3000], [new], 1024, 4)
+
+
+def test_sets_with_strided_queries_a_narrow_table_and_another_stream():
+    lens, new = [400, 77], [9, 3]
+    cache, table = filled_cache(35, lens, 2, 64, 512)
+    wide = queries(35, 12, 24, 512)
+    q = wide[:, 8:24]
+    want = attend(q.contiguous(), cache, table, lens, new)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = attend(q, cache, table, lens, new)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    out, _ = attend(q, cache, [row[:2] for row in table], lens, new)  # 128 tokens of 400
+    assert out[:9].isnan().all() and torch.equal(out[9:], want[0][9:])
+
+
+def test_sets_repeat_bitwise_in_a_graph():
+    lens, new = [3000, 500], [6, 4]
+    cache, table = filled_cache(36, lens, 4, 64, 512)
+    q = queries(36, 10, 32, 512)
+    tab, ln, cu = ints(table), ints(lens), ints(cu_of(new))
+
+    def call():
+        return g4.paged_cache_attention(q, cache, tab, ln, cu, max_seqlen_q=6, max_seqlen_k=3000)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(4):
+        q.copy_(queries(70 + i, 10, 32, 512))
+        ln.copy_(ints([3000 - 70 * i, 500 - i]))
+        graph.replay()
+        want = call()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
